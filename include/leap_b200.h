@@ -102,6 +102,25 @@ LEAP_API int leap_rope_table(int seq_len, int head_dim, float theta,
 LEAP_API int leap_ctx_create(const leap_ctx_desc *desc, leap_ctx **out);
 LEAP_API int leap_ctx_destroy(leap_ctx *ctx);
 
+/*
+ * The same with a choice of how K/V rows are kept:
+ *   LEAP_KV_F32  FP32 (leap_ctx_create);
+ *   LEAP_KV_Q8   8 bits: a row x of one kv head as head_dim codes of one byte
+ *                and an FP32 scale, s = max|x| * (1/127), c = x / s rounded to
+ *                the nearest integer (ties to even, within -127..127), which
+ *                stand for c * s.  head_dim 128: 132 bytes a row instead of 512.
+ *                A row holding an infinity or a NaN reads back as NaN.
+ * Every call below works on either kind (leap_attn_tree on LEAP_KV_Q8 only).
+ * With LEAP_KV_Q8, attention reads nothing but stored rows: a new token's own
+ * k (rotated as in the FP32 cache, then quantised) and v are appended first and
+ * read as they are kept.  Kernel selections (leap_set_decode_impl,
+ * leap_set_prefill_impl) concern LEAP_KV_F32.
+ */
+#define LEAP_KV_F32 0
+#define LEAP_KV_Q8 1
+LEAP_API int leap_ctx_create_kv(const leap_ctx_desc *desc, int kv_kind, leap_ctx **out);
+LEAP_API int leap_ctx_kv_kind(const leap_ctx *ctx, int *kv_kind);
+
 /* Use `stream` (a cudaStream_t; NULL = the CUDA default stream, as
  * everywhere in CUDA) for all following work of this context. */
 LEAP_API int leap_ctx_set_stream(leap_ctx *ctx, void *stream);
@@ -214,6 +233,54 @@ LEAP_API int leap_attn_prefill(leap_ctx *ctx, int slot, int layer, int pos0, int
                       float *out);
 
 /*
+ * Causal prefill of several prompts (or parts of prompts) taken together:
+ * sequence i brings n_tok[i] >= 0 tokens for slot slots[i], behind its pos0[i]
+ * cached rows; its token t sees rows 0..pos0[i]+t.  Semantics =
+ * leap_attn_prefill per sequence.
+ *   slots, pos0, n_tok: HOST int arrays of length n_seq; slots distinct
+ *   q [sum n_tok][n_heads][hd], k/v [sum n_tok][n_kv][hd] (un-rotated), the
+ *   sequences' tokens one after another; out like q.
+ */
+LEAP_API int leap_attn_prefill_packed(leap_ctx *ctx, int layer, int n_seq, const int *slots,
+                                      const int *pos0, const int *n_tok, const float *q,
+                                      const float *k, const float *v, float *out);
+
+/*
+ * Attention of drafted token trees over the cache (speculative decoding: all
+ * candidates of a step verified at once).  Sequence i brings n_nodes[i] nodes
+ * (0..128) behind its positions[i] cached rows.  parents[] (HOST, all
+ * sequences' nodes one after another) holds each node's parent within its
+ * sequence, -1 for none; a parent comes before its children.  A node at depth
+ * d (0 without a parent) is rotated for position positions[i] + d and sees the
+ * cached rows, its ancestors and itself.  Node j's k and v are appended as row
+ * positions[i] + j; leap_kv_keep then keeps the accepted path.
+ *   slots, positions, n_nodes, parents: HOST int arrays; slots distinct
+ *   q [sum n_nodes][n_heads][hd], k/v [sum n_nodes][n_kv][hd] (un-rotated)
+ */
+LEAP_API int leap_attn_tree(leap_ctx *ctx, int layer, int n_seq, const int *slots,
+                            const int *positions, const int *n_nodes, const int *parents,
+                            const float *q, const float *k, const float *v, float *out);
+
+/*
+ * Keep some of the rows that follow positions[i] in slot slots[i], in every
+ * layer of the context: row positions[i] + nodes[j] becomes row
+ * positions[i] + j, for sequence i's n_keep[i] (0..128) strictly increasing
+ * nodes (HOST, all sequences' one after another, each within 0..127).  After
+ * leap_attn_tree of every layer this keeps the accepted path (rows are rotated
+ * by depth already); later rows are left as they are, to be overwritten.
+ */
+LEAP_API int leap_kv_keep(leap_ctx *ctx, int n_seq, const int *slots, const int *positions,
+                          const int *n_keep, const int *nodes);
+
+/*
+ * Rows pos0[i] .. pos0[i]+n_tok[i]-1 of several slots of one layer, packed one
+ * sequence after another into DEVICE arrays k, v [sum n_tok][n_kv][hd], in one
+ * launch (leap_kv_read per sequence).
+ */
+LEAP_API int leap_kv_read_packed(leap_ctx *ctx, int layer, int n_seq, const int *slots,
+                                 const int *pos0, const int *n_tok, float *k, float *v);
+
+/*
  * Decode attention that allocates nothing.  (No counterpart in the
  * reference: LEAP's CPU engine owns all its memory in std::vectors.)
  *
@@ -299,6 +366,10 @@ LEAP_API int leap_engine_synthetic(const leap_model_config *cfg,
                                    int layer_begin, int layer_end,
                                    float rope_theta, int max_chunk,
                                    leap_engine **out);
+
+/* Replace the engine's KV cache by an empty one that keeps its rows as
+ * `kv_kind` says (leap_ctx_create_kv); engines are made with LEAP_KV_F32. */
+LEAP_API int leap_engine_set_kv(leap_engine *e, int kv_kind);
 
 LEAP_API int leap_engine_destroy(leap_engine *e);
 LEAP_API int leap_engine_config(const leap_engine *e, leap_model_config *cfg,

@@ -25,6 +25,9 @@ LEAP_ERR_DEVICE = 3
 LEAP_ERR_NOMEM = 4
 LEAP_ERR_COMM = 5
 
+LEAP_KV_F32 = 0
+LEAP_KV_Q8 = 1
+
 
 class CtxDesc(ctypes.Structure):
     """``leap_ctx_desc`` (include/leap_b200.h)."""
@@ -55,6 +58,8 @@ SIGNATURES: dict[str, tuple] = {
     "leap_version": (ctypes.c_char_p, []),
     "leap_rope_table": (c_int, [c_int, c_int, ctypes.c_float, c_float_p, c_float_p]),
     "leap_ctx_create": (c_int, [ctypes.POINTER(CtxDesc), ctypes.POINTER(c_void_p)]),
+    "leap_ctx_create_kv": (c_int, [ctypes.POINTER(CtxDesc), c_int, ctypes.POINTER(c_void_p)]),
+    "leap_ctx_kv_kind": (c_int, [c_void_p, c_int_p]),
     "leap_ctx_destroy": (c_int, [c_void_p]),
     "leap_ctx_set_stream": (c_int, [c_void_p, c_void_p]),
     "leap_ctx_use_own_stream": (c_int, [c_void_p]),
@@ -76,6 +81,11 @@ SIGNATURES: dict[str, tuple] = {
                                          c_void_p, c_void_p, c_void_p, c_void_p]),
     "leap_attn_prefill": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_void_p,
                                   c_void_p, c_void_p, c_void_p]),
+    # the ragged calls take their host int arrays as addresses
+    "leap_attn_prefill_packed": (c_int, [c_void_p, c_int, c_int] + [c_void_p] * 7),
+    "leap_attn_tree": (c_int, [c_void_p, c_int, c_int] + [c_void_p] * 8),
+    "leap_kv_keep": (c_int, [c_void_p, c_int] + [c_void_p] * 4),
+    "leap_kv_read_packed": (c_int, [c_void_p, c_int, c_int] + [c_void_p] * 5),
     "leap_set_prefill_impl": (c_int, [c_void_p, c_int]),
     "leap_attn_decode_noalloc": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_void_p,
                                          c_void_p, c_void_p, c_void_p, ctypes.c_longlong,
@@ -85,6 +95,7 @@ SIGNATURES: dict[str, tuple] = {
     "leap_engine_synthetic": (c_int, [ctypes.POINTER(ModelConfigC), ctypes.c_ulonglong, c_int,
                                       c_int, c_int, ctypes.c_float, c_int,
                                       ctypes.POINTER(c_void_p)]),
+    "leap_engine_set_kv": (c_int, [c_void_p, c_int]),
     "leap_engine_destroy": (c_int, [c_void_p]),
     "leap_engine_config": (c_int, [c_void_p, ctypes.POINTER(ModelConfigC), c_int_p, c_int_p]),
     "leap_engine_device_bytes": (c_int, [c_void_p, ctypes.POINTER(ctypes.c_size_t)]),

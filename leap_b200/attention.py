@@ -16,7 +16,7 @@ import ctypes
 
 import numpy as np
 
-from ._native import CtxDesc, LeapError, check, lib
+from ._native import LEAP_KV_F32, LEAP_KV_Q8, CtxDesc, LeapError, check, lib
 
 __all__ = ["AttentionContext", "LeapError", "rope_table"]
 
@@ -43,6 +43,23 @@ def _dptr(t) -> int:
     return t.data_ptr()
 
 
+KV_KINDS = {"f32": LEAP_KV_F32, "q8": LEAP_KV_Q8}
+
+
+def kv_kind(kv: str) -> int:
+    if kv not in KV_KINDS:
+        raise ValueError(f"kv must be one of {sorted(KV_KINDS)}, got {kv!r}")
+    return KV_KINDS[kv]
+
+
+def _ints(a, name: str, n: int | None = None) -> np.ndarray:
+    """A 1-D host int32 array (kept as it is when it is one already)."""
+    a = np.ascontiguousarray(a, np.int32)
+    if a.ndim != 1 or (n is not None and a.shape[0] != n):
+        raise ValueError(f"{name} must be 1-D" + ("" if n is None else f" of length {n}"))
+    return a
+
+
 def _hptr(a: np.ndarray) -> int:
     if a.dtype != np.float32 or not a.flags["C_CONTIGUOUS"]:
         raise TypeError("expected a C-contiguous float32 array")
@@ -56,12 +73,17 @@ class AttentionContext:
     ``n_heads``, ``n_kv_heads``, ``head_dim`` (= dim / n_heads), ``max_seq``
     (= seq_len).  ``rope_cos``/``rope_sin`` default to :func:`rope_table`
     with ``theta``.
+
+    ``kv`` says how cached rows are kept: ``"f32"``, or ``"q8"`` for 8-bit
+    codes with one scale for each row and kv head (``leap_ctx_create_kv``).
+    Every method works on both; :meth:`decode_tree` on ``"q8"`` only.
     """
 
     def __init__(self, n_layers: int, n_heads: int, n_kv_heads: int, head_dim: int,
                  max_seq: int, max_batch: int = 1, device: int = 0, layer0: int = 0,
                  theta: float = 500000.0, rope_cos=None, rope_sin=None,
-                 bind_torch_stream: bool = True):
+                 bind_torch_stream: bool = True, kv: str = "f32"):
+        kind = kv_kind(kv)
         if rope_cos is None or rope_sin is None:
             rope_cos, rope_sin = rope_table(max_seq, head_dim, theta)
         self.rope_cos = np.ascontiguousarray(rope_cos, np.float32)
@@ -73,11 +95,12 @@ class AttentionContext:
                        max_batch, device, self.rope_cos.ctypes.data_as(fp),
                        self.rope_sin.ctypes.data_as(fp))
         h = ctypes.c_void_p()
-        check(lib().leap_ctx_create(ctypes.byref(desc), ctypes.byref(h)))
+        check(lib().leap_ctx_create_kv(ctypes.byref(desc), kind, ctypes.byref(h)))
         self._h = h
         self.n_layers, self.n_heads, self.n_kv_heads = n_layers, n_heads, n_kv_heads
         self.head_dim, self.max_seq, self.max_batch = head_dim, max_seq, max_batch
         self.device = device
+        self.kv = kv
         if bind_torch_stream:
             self.bind_torch_stream()
 
@@ -151,6 +174,41 @@ class AttentionContext:
         check(lib().leap_kv_read(self.handle, slot, layer, pos0, n, _hptr(k), _hptr(v), 1))
         return k, v
 
+    def kv_read_device(self, slot: int, layer: int, pos0: int, n: int):
+        """The same as device tensors, on the context's stream."""
+        k, v = self._rows(n)
+        check(lib().leap_kv_read(self.handle, slot, layer, pos0, n, k.data_ptr(), v.data_ptr(), 0))
+        return k, v
+
+    def kv_read_packed(self, layer: int, slots, pos0, n_tok):
+        """Rows [pos0[i], pos0[i]+n_tok[i]) of slots[i], one sequence after
+        another, as device tensors [sum n_tok, n_kv, hd] (K, V): one launch."""
+        slots = _ints(slots, "slots")
+        n = slots.shape[0]
+        pos0, n_tok = _ints(pos0, "pos0", n), _ints(n_tok, "n_tok", n)
+        k, v = self._rows(int(n_tok.clip(0).sum()))
+        check(lib().leap_kv_read_packed(self.handle, layer, n, slots.ctypes.data,
+                                        pos0.ctypes.data, n_tok.ctypes.data, k.data_ptr(),
+                                        v.data_ptr()))
+        return k, v
+
+    def kv_keep(self, slots, positions, n_keep, nodes) -> None:
+        """Keep rows positions[i] + nodes (strictly increasing, n_keep[i] of
+        them for each sequence) as rows positions[i], positions[i]+1, ... in
+        every layer: the accepted path after :meth:`decode_tree`."""
+        slots = _ints(slots, "slots")
+        n = slots.shape[0]
+        positions, n_keep = _ints(positions, "positions", n), _ints(n_keep, "n_keep", n)
+        nodes = _ints(nodes, "nodes", int(n_keep.clip(0).sum()))
+        check(lib().leap_kv_keep(self.handle, n, slots.ctypes.data, positions.ctypes.data,
+                                 n_keep.ctypes.data, nodes.ctypes.data))
+
+    def _rows(self, n: int):
+        import torch
+        shape = (max(n, 0), self.n_kv_heads, self.head_dim)
+        return (torch.empty(shape, dtype=torch.float32, device=f"cuda:{self.device}"),
+                torch.empty(shape, dtype=torch.float32, device=f"cuda:{self.device}"))
+
     # -- attention ----------------------------------------------------------
     def decode(self, layer: int, pos: int, q, k_new, v_new, out=None):
         """Fused RoPE + append + attention for one token (device tensors)."""
@@ -195,6 +253,49 @@ class AttentionContext:
             out = torch.empty_like(q)
         check(lib().leap_attn_prefill(self.handle, slot, layer, pos0, int(q.shape[0]),
                                       _dptr(q), _dptr(k), _dptr(v), _dptr(out)))
+        return out
+
+    def _packed(self, total: int, q, k, v, out):
+        """Device pointers of a ragged call's tensors, their shapes checked."""
+        import torch
+        qs, ks = (total, self.n_heads, self.head_dim), (total, self.n_kv_heads, self.head_dim)
+        if out is None:
+            out = torch.empty_like(q)
+        ptrs = [_dptr(t) for t in (q, k, v, out)]
+        for name, t, shape in (("q", q, qs), ("k", k, ks), ("v", v, ks), ("out", out, qs)):
+            if tuple(t.shape) != shape:
+                raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+            if t.device.index != self.device:
+                raise ValueError(f"{name} must be on cuda:{self.device}, got {t.device}")
+        return (*ptrs, out)
+
+    def prefill_packed(self, layer: int, slots, pos0, n_tok, q, k, v, out=None):
+        """Causal prefill of several prompts (or parts of prompts): sequence i
+        brings n_tok[i] tokens for slots[i] behind pos0[i] cached rows; q, k, v
+        hold the sequences' tokens one after another."""
+        slots = _ints(slots, "slots")
+        n = slots.shape[0]
+        pos0, n_tok = _ints(pos0, "pos0", n), _ints(n_tok, "n_tok", n)
+        qp, kp, vp, op, out = self._packed(int(n_tok.clip(0).sum()), q, k, v, out)
+        check(lib().leap_attn_prefill_packed(self.handle, layer, n, slots.ctypes.data,
+                                             pos0.ctypes.data, n_tok.ctypes.data, qp, kp, vp, op))
+        return out
+
+    def decode_tree(self, layer: int, slots, positions, n_nodes, parents, q, k, v, out=None):
+        """Attention of drafted token trees: sequence i brings n_nodes[i] nodes
+        behind positions[i] cached rows.  ``parents`` holds each node's parent
+        within its sequence (-1: none; parents come before children), all
+        sequences' nodes one after another.  A node sees the cached rows, its
+        ancestors and itself; its k and v are appended as row positions[i] +
+        node.  ``kv="q8"`` only."""
+        slots = _ints(slots, "slots")
+        n = slots.shape[0]
+        positions, n_nodes = _ints(positions, "positions", n), _ints(n_nodes, "n_nodes", n)
+        total = int(n_nodes.clip(0).sum())
+        parents = _ints(parents, "parents", total)
+        qp, kp, vp, op, out = self._packed(total, q, k, v, out)
+        check(lib().leap_attn_tree(self.handle, layer, n, slots.ctypes.data, positions.ctypes.data,
+                                   n_nodes.ctypes.data, parents.ctypes.data, qp, kp, vp, op))
         return out
 
     def set_decode_impl(self, impl: int) -> None:

@@ -10,6 +10,7 @@
 #include <cstdint>
 #include <cstdio>
 #include <cstring>
+#include <memory>
 #include <new>
 #include <vector>
 
@@ -52,6 +53,7 @@ void free_ctx(leap_ctx *c) {
     if (c->stream && c->stream != c->own_stream) cudaStreamSynchronize(c->stream);
     cudaFree(c->k_cache);
     cudaFree(c->v_cache);
+    q8_free(c);
     cudaFree(c->rope_cos);
     cudaFree(c->rope_sin);
     for (int i = 0; i < 2; ++i) {
@@ -94,7 +96,8 @@ int check_device_error(leap_ctx *c) {
     // tickets and the error word so the next call starts clean.
     cudaMemset(c->d_err, 0, sizeof(int));
     for (int i = 0; i < 2; ++i)
-        cudaMemset(c->counters[i], 0, sizeof(unsigned) * kMaxSeqPerLaunch * c->n_kv);
+        if (c->counters[i])
+            cudaMemset(c->counters[i], 0, sizeof(unsigned) * kMaxSeqPerLaunch * c->n_kv);
     if (err == kDevErrBadToken)
         set_error("a device-side token id was outside [0, vocab_size)");
     else
@@ -167,12 +170,20 @@ int leap_rope_table(int seq_len, int head_dim, float theta, float *rope_cos, flo
 }
 
 int leap_ctx_create(const leap_ctx_desc *d, leap_ctx **out) {
+    return leap_ctx_create_kv(d, LEAP_KV_F32, out);
+}
+
+int leap_ctx_create_kv(const leap_ctx_desc *d, int kv_kind, leap_ctx **out) {
     leap::clear_error();
     if (!d || !out) {
         leap::set_error("null argument");
         return LEAP_ERR_INVALID;
     }
     *out = nullptr;
+    if (kv_kind != LEAP_KV_F32 && kv_kind != LEAP_KV_Q8) {
+        leap::set_error("kv kind %d unknown (LEAP_KV_F32 or LEAP_KV_Q8)", kv_kind);
+        return LEAP_ERR_INVALID;
+    }
     if (d->n_layers < 1 || d->n_heads < 1 || d->n_kv_heads < 1 ||
         d->n_heads % d->n_kv_heads != 0 || d->max_seq < 1 || d->max_batch < 1) {
         leap::set_error("invalid shape: n_layers %d n_heads %d n_kv_heads %d max_seq %d max_batch %d",
@@ -217,6 +228,7 @@ int leap_ctx_create(const leap_ctx_desc *d, leap_ctx **out) {
     c->max_seq = d->max_seq;
     c->max_seq_pad = (d->max_seq + 63) / 64 * 64;
     c->max_batch = d->max_batch;
+    c->kv_kind = kv_kind;
     int st = LEAP_OK;
     auto fail = [&](cudaError_t e, const char *what) {
         st = leap::cuda_status(e, what);
@@ -233,11 +245,19 @@ int leap_ctx_create(const leap_ctx_desc *d, leap_ctx **out) {
     if ((e = cudaStreamCreateWithFlags(&c->own_stream, cudaStreamNonBlocking)) != cudaSuccess)
         return fail(e, "cudaStreamCreate");
     c->stream = c->own_stream;
-    if ((e = cudaMalloc(&c->k_cache, c->cache_bytes)) != cudaSuccess) return fail(e, "cudaMalloc(k_cache)");
-    if ((e = cudaMalloc(&c->v_cache, c->cache_bytes)) != cudaSuccess) return fail(e, "cudaMalloc(v_cache)");
-    if ((e = cudaMemset(c->k_cache, 0, c->cache_bytes)) != cudaSuccess) return fail(e, "cudaMemset");
-    if ((e = cudaMemset(c->v_cache, 0, c->cache_bytes)) != cudaSuccess) return fail(e, "cudaMemset");
-    c->device_bytes += 2 * c->cache_bytes;
+    if (kv_kind == LEAP_KV_Q8) {
+        c->cache_bytes = 0;
+        if ((st = leap::q8_create(c)) != LEAP_OK) {
+            leap::free_ctx(c);
+            return st;
+        }
+    } else {
+        if ((e = cudaMalloc(&c->k_cache, c->cache_bytes)) != cudaSuccess) return fail(e, "cudaMalloc(k_cache)");
+        if ((e = cudaMalloc(&c->v_cache, c->cache_bytes)) != cudaSuccess) return fail(e, "cudaMalloc(v_cache)");
+        if ((e = cudaMemset(c->k_cache, 0, c->cache_bytes)) != cudaSuccess) return fail(e, "cudaMemset");
+        if ((e = cudaMemset(c->v_cache, 0, c->cache_bytes)) != cudaSuccess) return fail(e, "cudaMemset");
+        c->device_bytes += 2 * c->cache_bytes;
+    }
 
     const size_t rope_bytes = size_t(c->max_seq) * (c->hd / 2) * sizeof(float);
     if ((e = cudaMalloc(&c->rope_cos, rope_bytes)) != cudaSuccess) return fail(e, "cudaMalloc(rope)");
@@ -248,18 +268,20 @@ int leap_ctx_create(const leap_ctx_desc *d, leap_ctx **out) {
         return fail(e, "copy rope_sin");
     c->device_bytes += 2 * rope_bytes;
 
-    c->max_parts = leap::max_decode_parts(c->hd, c->n_kv, c->max_batch, c->max_seq_pad, c->num_sms);
-    const size_t po = size_t(c->max_parts) * c->group * c->hd * sizeof(float);
-    // (M, L) per head per partial, records padded to 16 bytes
-    const size_t pml = size_t(c->max_parts) * 2 * (c->group < 2 ? 2 : c->group) * sizeof(float);
-    const size_t cnt = size_t(leap::kMaxSeqPerLaunch) * c->n_kv * sizeof(unsigned);
-    for (int i = 0; i < 2; ++i) {
-        if ((e = cudaMalloc(&c->part_o[i], po)) != cudaSuccess) return fail(e, "cudaMalloc(partials)");
-        if ((e = cudaMalloc(&c->part_ml[i], pml)) != cudaSuccess) return fail(e, "cudaMalloc(partials)");
-        if ((e = cudaMalloc(&c->counters[i], cnt)) != cudaSuccess) return fail(e, "cudaMalloc(counters)");
-        if ((e = cudaMemset(c->counters[i], 0, cnt)) != cudaSuccess) return fail(e, "cudaMemset(counters)");
+    if (kv_kind == LEAP_KV_F32) {
+        c->max_parts = leap::max_decode_parts(c->hd, c->n_kv, c->max_batch, c->max_seq_pad, c->num_sms);
+        const size_t po = size_t(c->max_parts) * c->group * c->hd * sizeof(float);
+        // (M, L) per head per partial, records padded to 16 bytes
+        const size_t pml = size_t(c->max_parts) * 2 * (c->group < 2 ? 2 : c->group) * sizeof(float);
+        const size_t cnt = size_t(leap::kMaxSeqPerLaunch) * c->n_kv * sizeof(unsigned);
+        for (int i = 0; i < 2; ++i) {
+            if ((e = cudaMalloc(&c->part_o[i], po)) != cudaSuccess) return fail(e, "cudaMalloc(partials)");
+            if ((e = cudaMalloc(&c->part_ml[i], pml)) != cudaSuccess) return fail(e, "cudaMalloc(partials)");
+            if ((e = cudaMalloc(&c->counters[i], cnt)) != cudaSuccess) return fail(e, "cudaMalloc(counters)");
+            if ((e = cudaMemset(c->counters[i], 0, cnt)) != cudaSuccess) return fail(e, "cudaMemset(counters)");
+        }
+        c->device_bytes += 2 * (po + pml + cnt);
     }
-    c->device_bytes += 2 * (po + pml + cnt);
 
     const size_t sb = leap::stage_floats(c) * sizeof(float);
     if ((e = cudaMallocHost(&c->h_stage, sb)) != cudaSuccess) return fail(e, "cudaMallocHost(stage)");
@@ -332,6 +354,17 @@ int leap_set_overlap(leap_ctx *c, int enable) {
     return LEAP_OK;
 }
 
+int leap_ctx_kv_kind(const leap_ctx *c, int *kv_kind) {
+    leap::clear_error();
+    LEAP_CHECK_CTX(c);
+    if (!kv_kind) {
+        leap::set_error("null argument");
+        return LEAP_ERR_INVALID;
+    }
+    *kv_kind = c->kv_kind;
+    return LEAP_OK;
+}
+
 int leap_sync(leap_ctx *c) {
     leap::clear_error();
     LEAP_CHECK_CTX(c);
@@ -355,6 +388,7 @@ int leap_kv_clear(leap_ctx *c) {
     LEAP_CHECK_CTX(c);
     DeviceGuard g(c->device);
     c->last_written_layer = leap_ctx::kWroteAll;
+    if (c->kv_kind == LEAP_KV_Q8) return leap::q8_clear(c);
     LEAP_TRY_CUDA(cudaMemsetAsync(c->k_cache, 0, c->cache_bytes, c->stream), "clear k");
     LEAP_TRY_CUDA(cudaMemsetAsync(c->v_cache, 0, c->cache_bytes, c->stream), "clear v");
     return LEAP_OK;
@@ -382,6 +416,13 @@ int leap_kv_write(leap_ctx *c, int slot, int layer, int pos0, int n_pos, const f
     }
     DeviceGuard g(c->device);
     c->last_written_layer = leap_ctx::kWroteAll;
+    if (c->kv_kind == LEAP_KV_Q8) {
+        if (!from_host && (!leap::aligned16(k) || !leap::aligned16(v))) {
+            leap::set_error("k/v must be 16-byte aligned");
+            return LEAP_ERR_INVALID;
+        }
+        return leap::q8_write(c, slot, layer, pos0, n_pos, k, v, from_host != 0);
+    }
     const cudaMemcpyKind kind = from_host ? cudaMemcpyHostToDevice : cudaMemcpyDeviceToDevice;
     const size_t row = size_t(c->hd) * sizeof(float);
     for (int h = 0; h < c->n_kv; ++h) {
@@ -409,6 +450,13 @@ int leap_kv_read(leap_ctx *c, int slot, int layer, int pos0, int n_pos, float *k
         return LEAP_ERR_INVALID;
     }
     DeviceGuard g(c->device);
+    if (c->kv_kind == LEAP_KV_Q8) {
+        if (!to_host && (!leap::aligned16(k) || !leap::aligned16(v))) {
+            leap::set_error("k/v must be 16-byte aligned");
+            return LEAP_ERR_INVALID;
+        }
+        return leap::q8_read(c, slot, layer, pos0, n_pos, k, v, to_host != 0);
+    }
     const cudaMemcpyKind kind = to_host ? cudaMemcpyDeviceToHost : cudaMemcpyDeviceToDevice;
     const size_t row = size_t(c->hd) * sizeof(float);
     for (int h = 0; h < c->n_kv; ++h) {
@@ -443,6 +491,21 @@ static int decode_check(const leap_ctx *c, int layer, const float *q, const floa
     return LEAP_OK;
 }
 
+// One decode launch of tab's sequences over either kind of cache.
+static int decode_launch(leap_ctx *c, int layer, const leap::DecodeSeq &tab, const float *q,
+                         const float *k_new, const float *v_new, float *out) {
+    if (c->kv_kind != LEAP_KV_Q8) return leap::launch_decode(c, layer, tab, q, k_new, v_new, out);
+    leap::Q8Seqs s;
+    s.n_seq = tab.n_seq;
+    for (int i = 0; i < tab.n_seq; ++i) {
+        s.slot[i] = tab.slot[i];
+        s.pos[i] = tab.pos[i];
+        s.tok0[i] = i;
+    }
+    s.tok0[tab.n_seq] = tab.n_seq;
+    return leap::q8_attend(c, layer, s, nullptr, q, k_new, v_new, out);
+}
+
 int leap_attn_decode(leap_ctx *c, int layer, int pos, const float *q, const float *k_new,
                      const float *v_new, float *out) {
     leap::clear_error();
@@ -457,7 +520,7 @@ int leap_attn_decode(leap_ctx *c, int layer, int pos, const float *q, const floa
     tab.n_seq = 1;
     tab.pos[0] = pos;
     tab.slot[0] = 0;
-    return leap::launch_decode(c, layer, tab, q, k_new, v_new, out);
+    return decode_launch(c, layer, tab, q, k_new, v_new, out);
 }
 
 int leap_attn_decode_host(leap_ctx *c, int layer, int pos, const float *q, const float *k_new,
@@ -495,7 +558,7 @@ int leap_attn_decode_host(leap_ctx *c, int layer, int pos, const float *q, const
     tab.pos[0] = pos;
     tab.slot[0] = 0;
     c->err_host = reinterpret_cast<int *>(ho_dev + nq);
-    const int st = leap::launch_decode(c, layer, tab, dq, dk, dv, ho_dev);
+    const int st = decode_launch(c, layer, tab, dq, dk, dv, ho_dev);
     c->err_host = nullptr;
     if (st) return st;
     LEAP_TRY_CUDA(cudaStreamSynchronize(c->stream), "cudaStreamSynchronize");
@@ -536,12 +599,17 @@ int leap_attn_decode_batched(leap_ctx *c, int layer, int n_seq, const int *slots
             tab.pos[i] = positions[b0 + i];
             tab.slot[i] = slots[b0 + i];
         }
-            if (int st = leap::launch_decode(c, layer, tab, q + b0 * nq, k_new + b0 * nk,
-                                         v_new + b0 * nk, out + b0 * nq))
+        if (int st = decode_launch(c, layer, tab, q + b0 * nq, k_new + b0 * nk, v_new + b0 * nk,
+                                   out + b0 * nq))
             return st;
     }
     return LEAP_OK;
 }
+
+// Prefill launches of a checked ragged call over either kind of cache.
+static int prefill_launch(leap_ctx *c, int layer, const int *slots, const int *pos0,
+                          const int *n_tok, int n_seq, const float *q, const float *k,
+                          const float *v, float *out);
 
 int leap_attn_prefill(leap_ctx *c, int slot, int layer, int pos0, int n_tok, const float *q,
                       const float *k, const float *v, float *out) {
@@ -555,9 +623,212 @@ int leap_attn_prefill(leap_ctx *c, int slot, int layer, int pos0, int n_tok, con
     }
     if (n_tok == 0) return LEAP_OK;
     DeviceGuard g(c->device);
-    const int st = leap::launch_prefill(c, slot, layer, pos0, n_tok, q, k, v, out);
-    c->last_written_layer = layer;
-    return st;
+    return prefill_launch(c, layer, &slot, &pos0, &n_tok, 1, q, k, v, out);
+}
+
+// What every ragged call checks: each sequence's slot (distinct) and the rows
+// [pos0[i], pos0[i] + n[i]), n[i] <= most; *total = sum of n.
+static int ragged_check(const leap_ctx *c, int layer, int n_seq, const int *slots, const int *pos0,
+                        const int *n, int most, size_t *total) {
+    if (layer < 0 || layer >= c->n_layers) {
+        leap::set_error("layer %d out of range [0,%d)", layer, c->n_layers);
+        return LEAP_ERR_INVALID;
+    }
+    if (n_seq < 0 || (n_seq > 0 && (!slots || !pos0 || !n))) {
+        leap::set_error("bad n_seq / slots / positions / lengths");
+        return LEAP_ERR_INVALID;
+    }
+    // one bit a slot: on the stack for up to 1024 slots
+    uint64_t few[16] = {0};
+    std::unique_ptr<uint64_t[]> many;
+    uint64_t *seen = few;
+    if (c->max_batch > 1024) {
+        many.reset(new (std::nothrow) uint64_t[(c->max_batch + 63) / 64]());
+        if (!many) {
+            leap::set_error("host allocation failed");
+            return LEAP_ERR_NOMEM;
+        }
+        seen = many.get();
+    }
+    *total = 0;
+    for (int i = 0; i < n_seq; ++i) {
+        if (slots[i] < 0 || slots[i] >= c->max_batch || (seen[slots[i] >> 6] >> (slots[i] & 63) & 1)) {
+            leap::set_error("slot %d of sequence %d is out of range or repeated", slots[i], i);
+            return LEAP_ERR_INVALID;
+        }
+        seen[slots[i] >> 6] |= uint64_t(1) << (slots[i] & 63);
+        if (n[i] < 0 || n[i] > most || pos0[i] < 0 || pos0[i] > c->max_seq - n[i]) {
+            leap::set_error("sequence %d: %d tokens at %d (at most %d, max_seq %d)", i, n[i],
+                            pos0[i], most, c->max_seq);
+            return LEAP_ERR_INVALID;
+        }
+        *total += n[i];
+    }
+    if (*total * c->n_heads > size_t(INT32_MAX)) {
+        leap::set_error("too many tokens in one call");
+        return LEAP_ERR_INVALID;
+    }
+    return LEAP_OK;
+}
+
+// The next sequences of a ragged call, as many as one launch takes, from
+// sequence *i on (moved past them).
+static void next_seqs(leap::Q8Seqs &tab, int n_seq, const int *slots, const int *pos0, const int *n,
+                      int most_tokens, int *i) {
+    tab.n_seq = 0;
+    tab.tok0[0] = 0;
+    for (; *i < n_seq && tab.n_seq < leap::kMaxSeqPerLaunch; ++*i) {
+        const int t = tab.tok0[tab.n_seq];
+        if (most_tokens && t + n[*i] > most_tokens) break;
+        tab.slot[tab.n_seq] = slots[*i];
+        tab.pos[tab.n_seq] = pos0[*i];
+        tab.tok0[++tab.n_seq] = t + n[*i];
+    }
+}
+
+static int prefill_launch(leap_ctx *c, int layer, const int *slots, const int *pos0,
+                          const int *n_tok, int n_seq, const float *q, const float *k,
+                          const float *v, float *out) {
+    const size_t nq = size_t(c->n_heads) * c->hd, nk = size_t(c->n_kv) * c->hd;
+    for (int i = 0; i < n_seq;) {
+        size_t done;
+        int st;
+        if (c->kv_kind == LEAP_KV_Q8) {
+            leap::Q8Seqs tab;
+            next_seqs(tab, n_seq, slots, pos0, n_tok, 0, &i);
+            done = tab.tok0[tab.n_seq];
+            st = leap::q8_attend(c, layer, tab, nullptr, q, k, v, out);
+        } else {
+            done = n_tok[i];
+            st = done ? leap::launch_prefill(c, slots[i], layer, pos0[i], n_tok[i], q, k, v, out)
+                      : LEAP_OK;
+            ++i;
+        }
+        c->last_written_layer = layer;
+        if (st) return st;
+        q += done * nq;
+        k += done * nk;
+        v += done * nk;
+        out += done * nq;
+    }
+    return LEAP_OK;
+}
+
+int leap_attn_prefill_packed(leap_ctx *c, int layer, int n_seq, const int *slots, const int *pos0,
+                             const int *n_tok, const float *q, const float *k, const float *v,
+                             float *out) {
+    leap::clear_error();
+    LEAP_CHECK_CTX(c);
+    size_t total;
+    if (int st = ragged_check(c, layer, n_seq, slots, pos0, n_tok, c->max_seq, &total)) return st;
+    if (total == 0) return LEAP_OK;
+    if (int st = decode_check(c, layer, q, k, v, out)) return st;
+    DeviceGuard g(c->device);
+    return prefill_launch(c, layer, slots, pos0, n_tok, n_seq, q, k, v, out);
+}
+
+int leap_attn_tree(leap_ctx *c, int layer, int n_seq, const int *slots, const int *positions,
+                   const int *n_nodes, const int *parents, const float *q, const float *k,
+                   const float *v, float *out) {
+    leap::clear_error();
+    LEAP_CHECK_CTX(c);
+    if (c->kv_kind != LEAP_KV_Q8) {
+        leap::set_error("tree attention reads an 8-bit cache (leap_ctx_create_kv, LEAP_KV_Q8)");
+        return LEAP_ERR_INVALID;
+    }
+    size_t total;
+    if (int st = ragged_check(c, layer, n_seq, slots, positions, n_nodes, leap::kMaxTreeNodes, &total))
+        return st;
+    if (total == 0) return LEAP_OK;
+    if (!parents) {
+        leap::set_error("null parents");
+        return LEAP_ERR_INVALID;
+    }
+    if (int st = decode_check(c, layer, q, k, v, out)) return st;
+    const int *par = parents;
+    for (int i = 0; i < n_seq; par += n_nodes[i++])
+        for (int j = 0; j < n_nodes[i]; ++j)
+            if (par[j] < -1 || par[j] >= j) {
+                leap::set_error("sequence %d: parent %d of node %d is not an earlier node or -1", i,
+                                par[j], j);
+                return LEAP_ERR_INVALID;
+            }
+    DeviceGuard g(c->device);
+    const size_t nq = size_t(c->n_heads) * c->hd, nk = size_t(c->n_kv) * c->hd;
+    for (int i = 0; i < n_seq;) {
+        leap::Q8Seqs tab;
+        leap::Q8Tree tree;
+        next_seqs(tab, n_seq, slots, positions, n_nodes, leap::kMaxNodesPerLaunch, &i);
+        const int done = tab.tok0[tab.n_seq];
+        for (int j = 0; j < done; ++j) tree.parent[j] = int8_t(parents[j]);
+        const int st = leap::q8_attend(c, layer, tab, &tree, q, k, v, out);
+        c->last_written_layer = layer;
+        if (st) return st;
+        parents += done;
+        q += done * nq;
+        k += done * nk;
+        v += done * nk;
+        out += done * nq;
+    }
+    return LEAP_OK;
+}
+
+int leap_kv_keep(leap_ctx *c, int n_seq, const int *slots, const int *positions, const int *n_keep,
+                 const int *nodes) {
+    leap::clear_error();
+    LEAP_CHECK_CTX(c);
+    size_t total;
+    if (int st = ragged_check(c, 0, n_seq, slots, positions, n_keep, leap::kMaxTreeNodes, &total))
+        return st;
+    if (total == 0) return LEAP_OK;
+    if (!nodes) {
+        leap::set_error("null nodes");
+        return LEAP_ERR_INVALID;
+    }
+    const int *nd = nodes;
+    for (int i = 0; i < n_seq; nd += n_keep[i++])
+        for (int j = 0; j < n_keep[i]; ++j)
+            if (nd[j] < 0 || nd[j] >= leap::kMaxTreeNodes || (j > 0 && nd[j] <= nd[j - 1]) ||
+                nd[j] >= c->max_seq - positions[i]) {
+                leap::set_error("sequence %d: node %d is out of range or not above the one before", i,
+                                nd[j]);
+                return LEAP_ERR_INVALID;
+            }
+    DeviceGuard g(c->device);
+    c->last_written_layer = leap_ctx::kWroteAll;
+    for (int i = 0; i < n_seq;) {
+        leap::Q8Seqs tab;
+        leap::Q8Tree keep;
+        next_seqs(tab, n_seq, slots, positions, n_keep, leap::kMaxNodesPerLaunch, &i);
+        const int done = tab.tok0[tab.n_seq];
+        for (int j = 0; j < done; ++j) keep.parent[j] = int8_t(nodes[j]);
+        if (int st = leap::kv_keep(c, tab, keep)) return st;
+        nodes += done;
+    }
+    return LEAP_OK;
+}
+
+int leap_kv_read_packed(leap_ctx *c, int layer, int n_seq, const int *slots, const int *pos0,
+                        const int *n_tok, float *k, float *v) {
+    leap::clear_error();
+    LEAP_CHECK_CTX(c);
+    size_t total;
+    if (int st = ragged_check(c, layer, n_seq, slots, pos0, n_tok, c->max_seq, &total)) return st;
+    if (total == 0) return LEAP_OK;
+    if (!k || !v || !leap::aligned16(k) || !leap::aligned16(v)) {
+        leap::set_error("k/v must be non-null and 16-byte aligned");
+        return LEAP_ERR_INVALID;
+    }
+    DeviceGuard g(c->device);
+    for (int i = 0; i < n_seq;) {
+        leap::Q8Seqs tab;
+        next_seqs(tab, n_seq, slots, pos0, n_tok, 0, &i);
+        if (int st = leap::kv_read_packed(c, layer, tab, k, v)) return st;
+        const size_t done = size_t(tab.tok0[tab.n_seq]) * c->n_kv * c->hd;
+        k += done;
+        v += done;
+    }
+    return LEAP_OK;
 }
 
 int leap_set_prefill_impl(leap_ctx *c, int impl) {

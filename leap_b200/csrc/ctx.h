@@ -25,6 +25,15 @@ struct leap_ctx {
     size_t head_stride = 0, layer_stride = 0, slot_stride = 0;
     size_t cache_bytes = 0;  // per tensor (K or V)
 
+    // 8-bit cache (kv_kind LEAP_KV_Q8; format in q8.cuh): codes in the layout
+    // of the FP32 cache with one byte a value, one scale for each row; the
+    // strides below count rows
+    int kv_kind = LEAP_KV_F32;
+    uint8_t *k8 = nullptr, *v8 = nullptr;
+    float *ks8 = nullptr, *vs8 = nullptr;
+    size_t head_rows = 0, layer_rows = 0, slot_rows = 0;
+    float *d_rows = nullptr;  // FP32 rows on their way from or to host memory
+
     // RoPE table [max_seq][hd/2]
     float *rope_cos = nullptr, *rope_sin = nullptr;
 
@@ -133,5 +142,48 @@ int max_decode_parts(int hd, int n_kv, int max_batch, int max_seq_pad, int num_s
 // ---- prefill attention (prefill_attn.cu) ---------------------------------
 int launch_prefill(leap_ctx *c, int slot, int layer, int pos0, int n_tok,
                    const float *q, const float *k, const float *v, float *out);
+
+// ---- 8-bit KV cache (kv_q8.cu, attn_q8*.cu) --------------------------------
+constexpr int kMaxTreeNodes = 128;     // nodes of one sequence's tree
+constexpr int kMaxNodesPerLaunch = 4096;
+constexpr int kQ8StageRows = 1024;     // rows of k and v that d_rows holds
+
+// A ragged batch of new tokens, by value in kernel parameters: sequence i has
+// packed tokens tok0[i] .. tok0[i+1]-1 behind pos[i] cached rows of its slot.
+struct Q8Seqs {
+    int n_seq;
+    int slot[kMaxSeqPerLaunch];
+    int pos[kMaxSeqPerLaunch];
+    int tok0[kMaxSeqPerLaunch + 1];
+};
+// Parent of each packed token, counted from its sequence's first; -1: none.
+struct Q8Tree {
+    int8_t parent[kMaxNodesPerLaunch];
+};
+
+// One layer of the cache as kernels see it.
+struct Q8Layer {
+    uint8_t *k, *v;    // codes of (slot 0, this layer, kv head 0)
+    float *ks, *vs;    // scales
+    size_t head_rows, slot_rows;
+    int n_kv;
+};
+Q8Layer q8_layer(const leap_ctx *c, int layer);
+
+int q8_create(leap_ctx *c);
+void q8_free(leap_ctx *c);
+int q8_clear(leap_ctx *c);
+int q8_write(leap_ctx *c, int slot, int layer, int pos0, int n, const float *k, const float *v,
+             bool from_host);
+int q8_read(leap_ctx *c, int slot, int layer, int pos0, int n, float *k, float *v, bool to_host);
+// Rotate (tree: by depth), quantise and append every token's k and v.
+int q8_append(leap_ctx *c, int layer, const Q8Seqs &tab, const Q8Tree *tree, const float *k,
+              const float *v);
+int kv_read_packed(leap_ctx *c, int layer, const Q8Seqs &tab, float *k, float *v);
+// Move rows pos + node[j] to pos + j (j counted from each sequence's first).
+int kv_keep(leap_ctx *c, const Q8Seqs &tab, const Q8Tree &nodes);
+// Append and attend: causal, or a tree of each sequence's tokens.
+int q8_attend(leap_ctx *c, int layer, const Q8Seqs &tab, const Q8Tree *tree, const float *q,
+              const float *k, const float *v, float *out);
 
 }  // namespace leap

@@ -213,7 +213,9 @@ int allocate(leap_engine *e) {
     return LEAP_OK;
 }
 
-int make_attention(leap_engine *e, float theta) {
+// The engine's attention context, made (again) with a cache of kv_kind.  The
+// one it had goes only once the new one is there.
+int make_attention(leap_engine *e, float theta, int kv_kind = LEAP_KV_F32) {
     const leap_model_config &c = e->cfg;
     std::vector<float> rc(size_t(c.seq_len) * (e->head_dim / 2)), rs(rc.size());
     ETRY(leap_rope_table(c.seq_len, e->head_dim, theta, rc.data(), rs.data()));
@@ -228,11 +230,19 @@ int make_attention(leap_engine *e, float theta) {
     d.device = e->device;
     d.rope_cos = rc.data();
     d.rope_sin = rs.data();
-    ETRY(leap_ctx_create(&d, &e->attn));
-    ETRY(leap_ctx_set_stream(e->attn, e->stream));
+    leap_ctx *fresh = nullptr;
+    ETRY(leap_ctx_create_kv(&d, kv_kind, &fresh));
     size_t b = 0;
+    if (e->attn) {
+        leap_ctx_device_bytes(e->attn, &b);
+        e->device_bytes -= b;
+        leap_ctx_destroy(e->attn);  // waits for its stream
+    }
+    e->attn = fresh;
+    ETRY(leap_ctx_set_stream(e->attn, e->stream));
     leap_ctx_device_bytes(e->attn, &b);
     e->device_bytes += b;
+    e->rope_theta = theta;
     return LEAP_OK;
 }
 
@@ -624,6 +634,16 @@ int leap_engine_synthetic(const leap_model_config *cfg, unsigned long long seed,
     }
     *out = e;
     return LEAP_OK;
+}
+
+int leap_engine_set_kv(leap_engine *e, int kv_kind) {
+    leap::clear_error();
+    if (!e || (kv_kind != LEAP_KV_F32 && kv_kind != LEAP_KV_Q8)) {
+        leap::set_error("engine set_kv: null engine or unknown kv kind %d", kv_kind);
+        return LEAP_ERR_INVALID;
+    }
+    DevGuard g(e->device);
+    return make_attention(e, e->rope_theta, kv_kind);
 }
 
 int leap_engine_destroy(leap_engine *e) {

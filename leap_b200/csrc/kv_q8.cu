@@ -1,0 +1,320 @@
+// kv_q8.cu — rows into and out of the 8-bit KV cache: quantise (with or
+// without the rotation), read back, and the compaction after a verified tree.
+//
+// All of it is bound by HBM: a row of K and V of one kv head is 8*HD bytes of
+// FP32 on one side and 2*(HD + 4) bytes on the other.  One warp takes one
+// (token, kv head): a lane holds HD/32 neighbouring dims of k and of v (a
+// rotation pair never leaves a lane), the row's maximum is one warp reduction,
+// and each row is stored as one 128-byte (or 64-byte) line.  Nothing is staged
+// in shared memory; with 8 warps a block and 8 blocks an SM, 64 KB of loads
+// are in flight on each SM.
+#include "q8.cuh"
+
+namespace leap {
+namespace {
+
+constexpr int kWarps = 8;  // warps of a block
+
+enum { kRaw = 0, kCausal = 1, kTree = 2 };  // what the append kernel rotates by
+
+template <int HD>
+struct Vec;
+template <> struct Vec<128> { using T = float4; };
+template <> struct Vec<64> { using T = float2; };
+
+// MODE kRaw: rows as they are; kCausal: k rotated for its row's position;
+// kTree: k rotated for position pos + depth.
+template <int HD, int MODE>
+__global__ void __launch_bounds__(32 * kWarps)
+q8_append_kernel(const float *__restrict__ k, const float *__restrict__ v, const Q8Layer L,
+                 const float *__restrict__ rope_cos, const float *__restrict__ rope_sin,
+                 const __grid_constant__ Q8Seqs tab, const __grid_constant__ Q8Tree tree) {
+    constexpr int E = HD / 32;
+    grid_launch_dependents();  // what follows waits for this grid before it reads
+    const int lane = threadIdx.x & 31;
+    const int item = blockIdx.x * kWarps + (threadIdx.x >> 5);
+    const int total = tab.tok0[tab.n_seq];
+    if (item >= total * L.n_kv) return;
+    const int t = item / L.n_kv, h = item - t * L.n_kv;
+    const int seq = q8_seq_of(tab, t);
+    const int i = t - tab.tok0[seq];
+    const int row = tab.pos[seq] + i;
+    using V = typename Vec<HD>::T;
+    const V kx = *reinterpret_cast<const V *>(k + size_t(item) * HD + E * lane);
+    const V vx = *reinterpret_cast<const V *>(v + size_t(item) * HD + E * lane);
+    float x[E], y[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        x[e] = reinterpret_cast<const float *>(&kx)[e];
+        y[e] = reinterpret_cast<const float *>(&vx)[e];
+    }
+    if (MODE != kRaw) {
+        int at = row;
+        if (MODE == kTree) {
+            at = tab.pos[seq];
+            const int8_t *parent = tree.parent + tab.tok0[seq];
+            for (int p = parent[i]; p >= 0; p = parent[p]) ++at;  // parents come before children
+        }
+        const float *rc = rope_cos + size_t(at) * (HD / 2) + lane * (E / 2);
+        const float *rs = rope_sin + size_t(at) * (HD / 2) + lane * (E / 2);
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+            const float2 r = rope_pair(x[e], x[e + 1], rc[e / 2], rs[e / 2]);
+            x[e] = r.x;
+            x[e + 1] = r.y;
+        }
+    }
+    const size_t r0 = tab.slot[seq] * L.slot_rows + h * L.head_rows;
+    uint32_t c;
+    const float sk = q8_quantize<E>(x, c);
+    q8_store_codes<HD>(L.k + r0 * HD, row, lane, c);
+    const float sv = q8_quantize<E>(y, c);
+    q8_store_codes<HD>(L.v + r0 * HD, row, lane, c);
+    if (lane == 0) {
+        L.ks[r0 + row] = sk;
+        L.vs[r0 + row] = sv;
+    }
+}
+
+template <int HD>
+__global__ void __launch_bounds__(32 * kWarps)
+q8_read_kernel(float *__restrict__ k, float *__restrict__ v, const Q8Layer L,
+               const __grid_constant__ Q8Seqs tab) {
+    constexpr int E = HD / 32;
+    const int lane = threadIdx.x & 31;
+    const int item = blockIdx.x * kWarps + (threadIdx.x >> 5);
+    if (item >= tab.tok0[tab.n_seq] * L.n_kv) return;
+    const int t = item / L.n_kv, h = item - t * L.n_kv;
+    const int seq = q8_seq_of(tab, t);
+    const int row = tab.pos[seq] + t - tab.tok0[seq];
+    const size_t r0 = tab.slot[seq] * L.slot_rows + h * L.head_rows;
+    const uint32_t ck = q8_load_codes<HD>(L.k + r0 * HD, row, lane);
+    const uint32_t cv = q8_load_codes<HD>(L.v + r0 * HD, row, lane);
+    const float sk = L.ks[r0 + row], sv = L.vs[r0 + row];
+    using V = typename Vec<HD>::T;
+    V x, y;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        reinterpret_cast<float *>(&x)[e] = float(int((ck >> (8 * e)) & 255u) - 128) * sk;
+        reinterpret_cast<float *>(&y)[e] = float(int((cv >> (8 * e)) & 255u) - 128) * sv;
+    }
+    *reinterpret_cast<V *>(k + size_t(item) * HD + E * lane) = x;
+    *reinterpret_cast<V *>(v + size_t(item) * HD + E * lane) = y;
+}
+
+// The same from an FP32 cache.
+__global__ void __launch_bounds__(256)
+f32_read_kernel(float *__restrict__ k, float *__restrict__ v, const float *__restrict__ kc,
+                const float *__restrict__ vc, size_t head_stride, size_t slot_stride, int n_kv,
+                int hd4, const __grid_constant__ Q8Seqs tab) {
+    const long n = long(tab.tok0[tab.n_seq]) * n_kv * hd4;
+    const long f = blockIdx.x * 256L + threadIdx.x;
+    if (f >= n) return;
+    const int item = int(f / hd4), d = int(f % hd4);
+    const int t = item / n_kv, h = item - t * n_kv;
+    const int seq = q8_seq_of(tab, t);
+    const size_t src = tab.slot[seq] * slot_stride + h * head_stride +
+                       (size_t(tab.pos[seq] + t - tab.tok0[seq]) * hd4 + d) * 4;
+    reinterpret_cast<float4 *>(k)[f] = *reinterpret_cast<const float4 *>(kc + src);
+    reinterpret_cast<float4 *>(v)[f] = *reinterpret_cast<const float4 *>(vc + src);
+}
+
+// Keep rows pos + node[j] as pos + j.  A thread moves the same dims of every
+// row, in order of j; node[] increases strictly, so a row is read before
+// anything is written to it (node[j] >= j), also when kBatch rows are read
+// ahead of their writes.  Block: (sequence, layer, kv head); T: what a thread
+// moves of a K or V row (RowOff: where that lies in row r).
+constexpr int kBatch = 8;
+template <typename T, typename RowOff>
+__device__ __forceinline__ void keep_rows(T *head, int n, int pos, const int8_t *node, RowOff off) {
+    for (int j0 = 0; j0 < n; j0 += kBatch) {
+        T x[kBatch];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u)
+            if (j0 + u < n) x[u] = head[off(pos + node[j0 + u])];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u)
+            if (j0 + u < n) head[off(pos + j0 + u)] = x[u];
+    }
+}
+
+template <int HD>
+__global__ void __launch_bounds__(96)
+q8_keep_kernel(const Q8Layer L, size_t layer_rows, const __grid_constant__ Q8Seqs tab,
+               const __grid_constant__ Q8Tree nodes) {
+    const int seq = blockIdx.x, h = blockIdx.z;
+    const int t0 = tab.tok0[seq], n = tab.tok0[seq + 1] - t0, pos = tab.pos[seq];
+    const int8_t *node = nodes.parent + t0;
+    const size_t r0 = tab.slot[seq] * L.slot_rows + blockIdx.y * layer_rows + h * L.head_rows;
+    const int lane = threadIdx.x & 31, what = threadIdx.x >> 5;
+    using T = typename std::conditional<HD == 128, uint32_t, uint16_t>::type;
+    if (what < 2) {  // a warp each for the codes of K and of V
+        keep_rows(reinterpret_cast<T *>((what ? L.v : L.k) + r0 * HD), n, pos, node, [lane](int r) {
+            return HD == 128 ? q8_chunk<HD>(r, lane >> 2) / 4 + (lane & 3)
+                             : q8_chunk<HD>(r, lane >> 3) / 2 + (lane & 7);
+        });
+    } else if (lane < 2) {  // a thread each for the scales
+        keep_rows((lane ? L.vs : L.ks) + r0, n, pos, node, [](int r) { return size_t(r); });
+    }
+}
+
+__global__ void __launch_bounds__(64)
+f32_keep_kernel(float *kc, float *vc, size_t head_stride, size_t layer_stride, size_t slot_stride,
+                int hd4, const __grid_constant__ Q8Seqs tab, const __grid_constant__ Q8Tree nodes) {
+    const int seq = blockIdx.x;
+    const int t0 = tab.tok0[seq], n = tab.tok0[seq + 1] - t0;
+    const int lane = threadIdx.x & 31;
+    float *head = ((threadIdx.x >> 5) ? vc : kc) + tab.slot[seq] * slot_stride +
+                  blockIdx.y * layer_stride + blockIdx.z * head_stride;
+    if (lane < hd4)
+        keep_rows(reinterpret_cast<float4 *>(head), n, tab.pos[seq], nodes.parent + t0,
+                  [lane, hd4](int r) { return size_t(r) * hd4 + lane; });
+}
+
+template <int HD, int MODE>
+int launch_append(leap_ctx *c, int layer, const Q8Seqs &tab, const Q8Tree *tree, const float *k,
+                  const float *v) {
+    static const Q8Tree none = {};
+    const int items = tab.tok0[tab.n_seq] * c->n_kv;
+    if (items == 0) return LEAP_OK;
+    q8_append_kernel<HD, MODE><<<(items + kWarps - 1) / kWarps, 32 * kWarps, 0, c->stream>>>(
+        k, v, q8_layer(c, layer), c->rope_cos, c->rope_sin, tab, tree ? *tree : none);
+    return cuda_status(cudaGetLastError(), "q8_append_kernel launch");
+}
+
+int launch_read(leap_ctx *c, int layer, const Q8Seqs &tab, float *k, float *v) {
+    const int items = tab.tok0[tab.n_seq] * c->n_kv;
+    if (items == 0) return LEAP_OK;
+    const int grid = (items + kWarps - 1) / kWarps;
+    if (c->hd == 128)
+        q8_read_kernel<128><<<grid, 32 * kWarps, 0, c->stream>>>(k, v, q8_layer(c, layer), tab);
+    else
+        q8_read_kernel<64><<<grid, 32 * kWarps, 0, c->stream>>>(k, v, q8_layer(c, layer), tab);
+    return cuda_status(cudaGetLastError(), "q8_read_kernel launch");
+}
+
+Q8Seqs one_run(int slot, int pos0, int n) {
+    Q8Seqs tab;
+    tab.n_seq = 1;
+    tab.slot[0] = slot;
+    tab.pos[0] = pos0;
+    tab.tok0[0] = 0;
+    tab.tok0[1] = n;
+    return tab;
+}
+
+int write_rows(leap_ctx *c, int layer, const Q8Seqs &tab, const float *k, const float *v) {
+    return c->hd == 128 ? launch_append<128, kRaw>(c, layer, tab, nullptr, k, v)
+                        : launch_append<64, kRaw>(c, layer, tab, nullptr, k, v);
+}
+
+}  // namespace
+
+Q8Layer q8_layer(const leap_ctx *c, int layer) {
+    const size_t r = layer * c->layer_rows;
+    return {c->k8 + r * c->hd, c->v8 + r * c->hd, c->ks8 + r, c->vs8 + r,
+            c->head_rows,      c->slot_rows,      c->n_kv};
+}
+
+int q8_create(leap_ctx *c) {
+    c->head_rows = c->max_seq_pad;
+    c->layer_rows = c->n_kv * c->head_rows;
+    c->slot_rows = c->n_layers * c->layer_rows;
+    const size_t rows = c->max_batch * c->slot_rows;
+    const size_t stage = 2 * sizeof(float) * kQ8StageRows * c->n_kv * c->hd;
+    cudaError_t e = cudaMalloc(&c->k8, rows * c->hd);
+    if (e == cudaSuccess) e = cudaMalloc(&c->v8, rows * c->hd);
+    if (e == cudaSuccess) e = cudaMalloc(&c->ks8, rows * sizeof(float));
+    if (e == cudaSuccess) e = cudaMalloc(&c->vs8, rows * sizeof(float));
+    if (e == cudaSuccess) e = cudaMalloc(&c->d_rows, stage);
+    if (e != cudaSuccess) return cuda_status(e, "cudaMalloc(8-bit cache)");
+    c->device_bytes += 2 * rows * (c->hd + sizeof(float)) + stage;
+    return q8_clear(c);
+}
+
+void q8_free(leap_ctx *c) {
+    cudaFree(c->k8);
+    cudaFree(c->v8);
+    cudaFree(c->ks8);
+    cudaFree(c->vs8);
+    cudaFree(c->d_rows);
+}
+
+int q8_clear(leap_ctx *c) {
+    // code 128 stands for 0; with scale 0 every row reads as zeros
+    const size_t rows = c->max_batch * c->slot_rows;
+    cudaError_t e = cudaMemsetAsync(c->k8, 128, rows * c->hd, c->stream);
+    if (e == cudaSuccess) e = cudaMemsetAsync(c->v8, 128, rows * c->hd, c->stream);
+    if (e == cudaSuccess) e = cudaMemsetAsync(c->ks8, 0, rows * sizeof(float), c->stream);
+    if (e == cudaSuccess) e = cudaMemsetAsync(c->vs8, 0, rows * sizeof(float), c->stream);
+    return cuda_status(e, "clear the 8-bit cache");
+}
+
+int q8_write(leap_ctx *c, int slot, int layer, int pos0, int n, const float *k, const float *v,
+             bool from_host) {
+    if (!from_host) return write_rows(c, layer, one_run(slot, pos0, n), k, v);
+    const size_t row = size_t(c->n_kv) * c->hd;
+    float *dk = c->d_rows, *dv = dk + kQ8StageRows * row;
+    for (int r = 0; r < n; r += kQ8StageRows) {
+        const int m = n - r < kQ8StageRows ? n - r : kQ8StageRows;
+        const size_t bytes = m * row * sizeof(float);
+        cudaError_t e = cudaMemcpyAsync(dk, k + r * row, bytes, cudaMemcpyHostToDevice, c->stream);
+        if (e == cudaSuccess)
+            e = cudaMemcpyAsync(dv, v + r * row, bytes, cudaMemcpyHostToDevice, c->stream);
+        if (int st = cuda_status(e, "kv_write copy")) return st;
+        if (int st = write_rows(c, layer, one_run(slot, pos0 + r, m), dk, dv)) return st;
+    }
+    return cuda_status(cudaStreamSynchronize(c->stream), "kv_write sync");
+}
+
+int q8_read(leap_ctx *c, int slot, int layer, int pos0, int n, float *k, float *v, bool to_host) {
+    if (!to_host) return launch_read(c, layer, one_run(slot, pos0, n), k, v);
+    const size_t row = size_t(c->n_kv) * c->hd;
+    float *dk = c->d_rows, *dv = dk + kQ8StageRows * row;
+    for (int r = 0; r < n; r += kQ8StageRows) {
+        const int m = n - r < kQ8StageRows ? n - r : kQ8StageRows;
+        const size_t bytes = m * row * sizeof(float);
+        if (int st = launch_read(c, layer, one_run(slot, pos0 + r, m), dk, dv)) return st;
+        cudaError_t e = cudaMemcpyAsync(k + r * row, dk, bytes, cudaMemcpyDeviceToHost, c->stream);
+        if (e == cudaSuccess)
+            e = cudaMemcpyAsync(v + r * row, dv, bytes, cudaMemcpyDeviceToHost, c->stream);
+        if (int st = cuda_status(e, "kv_read copy")) return st;
+    }
+    return cuda_status(cudaStreamSynchronize(c->stream), "kv_read sync");
+}
+
+int q8_append(leap_ctx *c, int layer, const Q8Seqs &tab, const Q8Tree *tree, const float *k,
+              const float *v) {
+    if (c->hd == 128)
+        return tree ? launch_append<128, kTree>(c, layer, tab, tree, k, v)
+                    : launch_append<128, kCausal>(c, layer, tab, nullptr, k, v);
+    return tree ? launch_append<64, kTree>(c, layer, tab, tree, k, v)
+                : launch_append<64, kCausal>(c, layer, tab, nullptr, k, v);
+}
+
+int kv_read_packed(leap_ctx *c, int layer, const Q8Seqs &tab, float *k, float *v) {
+    if (c->kv_kind == LEAP_KV_Q8) return launch_read(c, layer, tab, k, v);
+    const long n = long(tab.tok0[tab.n_seq]) * c->n_kv * (c->hd / 4);
+    if (n == 0) return LEAP_OK;
+    f32_read_kernel<<<unsigned((n + 255) / 256), 256, 0, c->stream>>>(
+        k, v, k_head_ptr(c, 0, layer, 0), v_head_ptr(c, 0, layer, 0), c->head_stride,
+        c->slot_stride, c->n_kv, c->hd / 4, tab);
+    return cuda_status(cudaGetLastError(), "f32_read_kernel launch");
+}
+
+int kv_keep(leap_ctx *c, const Q8Seqs &tab, const Q8Tree &nodes) {
+    const dim3 grid(tab.n_seq, c->n_layers, c->n_kv);
+    if (c->kv_kind != LEAP_KV_Q8) {
+        f32_keep_kernel<<<grid, 64, 0, c->stream>>>(c->k_cache, c->v_cache, c->head_stride,
+                                                    c->layer_stride, c->slot_stride, c->hd / 4,
+                                                    tab, nodes);
+        return cuda_status(cudaGetLastError(), "f32_keep_kernel launch");
+    }
+    if (c->hd == 128)
+        q8_keep_kernel<128><<<grid, 96, 0, c->stream>>>(q8_layer(c, 0), c->layer_rows, tab, nodes);
+    else
+        q8_keep_kernel<64><<<grid, 96, 0, c->stream>>>(q8_layer(c, 0), c->layer_rows, tab, nodes);
+    return cuda_status(cudaGetLastError(), "q8_keep_kernel launch");
+}
+
+}  // namespace leap

@@ -1,0 +1,95 @@
+// q8.cuh — the 8-bit KV cache: row format, batch tables, device helpers.
+//
+// A row x[HD] of one kv head is stored as HD codes of one byte and one FP32
+// scale:  s = max|x| * (1/127),  c = x / s rounded to the nearest integer
+// (ties to even, within -127..127); it stands for c * s.  Codes are stored
+// plus 128 (1..255), so that one byte permute per two codes builds FP16 pairs
+// (0x6400 | u is 1024 + u).  A row that holds an infinity or a NaN gets codes
+// 0 and a NaN scale: it reads back as NaN, and what attends to it is NaN.
+//
+// Layout: codes [slot][layer][kv_head][max_seq_pad][HD], scales
+// [slot][layer][kv_head][max_seq_pad], so a run of rows is one contiguous
+// bulk copy of each.  Inside a 128-byte line (one row of 128, two rows of 64)
+// the 16-byte chunks are permuted by the row index (q8_chunk below): a linear
+// copy into shared memory then serves both fragment patterns of mma.sync
+// without bank conflicts (eight consecutive rows read at two chunk halves for
+// K, rows 2t / 2t+1 read at neighbouring chunks for V).
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+#include "ctx.h"
+
+namespace leap {
+
+// Byte offset, from the first row of a head, of 16-byte chunk `c` of row `r`.
+template <int HD>
+__host__ __device__ __forceinline__ size_t q8_chunk(int r, int c) {
+    if (HD == 128)
+        return size_t(r) * 128 + (unsigned(c ^ ((((r >> 1) & 3) << 1) ^ ((r & 1) << 2))) << 4);
+    const int line = r >> 1;
+    return size_t(line) * 128 + (unsigned((((r & 1) << 2) | c) ^ ((line & 3) << 1)) << 4);
+}
+
+// Sequence of packed token `t`: the last i with tok0[i] <= t (sequences
+// without tokens are stepped over, since their tok0 equals the next one's).
+__device__ __forceinline__ int q8_seq_of(const Q8Seqs &tab, int t) {
+    int lo = 0, hi = tab.n_seq - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (tab.tok0[mid] <= t) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+}
+
+// The code nearest to x / s (ties to even), `s` normal and inv near 1 / s:
+// the rounded product is at most one off, and the residual x - q*s, exact in
+// one fused multiply-add, tells on which side of the half x lies.
+__device__ __forceinline__ int q8_code(float x, float s, float inv) {
+    float q = rintf(x * inv);
+    const float r = fmaf(-q, s, x);
+    const float a = fabsf(r), half = 0.5f * s;
+    if (a > half || (a == half && (int(q) & 1))) q += r > 0.f ? 1.f : -1.f;
+    return int(fminf(fmaxf(q, -127.f), 127.f));
+}
+
+// One warp quantises one row, lane l holding x[E] = dims E*l .. E*l+E-1.
+// Returns the scale (the same in every lane) and this lane's codes + 128, the
+// lowest dim in the lowest byte.
+template <int E>
+__device__ __forceinline__ float q8_quantize(const float (&x)[E], uint32_t &codes) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+    top = __reduce_max_sync(0xffffffffu, top);
+    codes = E == 4 ? 0x80808080u : 0x8080u;
+    if (top >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
+    const float s = __fmul_rn(__uint_as_float(top), 1.0f / 127.0f);
+    if (s == 0.f) return 0.f;
+    // tiny rows: x and s by 2^64 (exact), so that 1/s stays finite
+    const float up = top < 0x21800000u /* 2^-60 */ ? 18446744073709551616.f : 1.f;
+    const float su = s * up, inv = 1.0f / su;
+    codes = 0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) codes |= uint32_t(q8_code(x[i] * up, su, inv) + 128) << (8 * i);
+    return s;
+}
+
+// Store / load a lane's codes (E = HD / 32 of them) of row r.
+template <int HD>
+__device__ __forceinline__ void q8_store_codes(uint8_t *head, int r, int lane, uint32_t codes) {
+    if (HD == 128)
+        *reinterpret_cast<uint32_t *>(head + q8_chunk<HD>(r, lane >> 2) + (lane & 3) * 4) = codes;
+    else
+        *reinterpret_cast<uint16_t *>(head + q8_chunk<HD>(r, lane >> 3) + (lane & 7) * 2) =
+            uint16_t(codes);
+}
+template <int HD>
+__device__ __forceinline__ uint32_t q8_load_codes(const uint8_t *head, int r, int lane) {
+    if (HD == 128)
+        return *reinterpret_cast<const uint32_t *>(head + q8_chunk<HD>(r, lane >> 2) + (lane & 3) * 4);
+    return *reinterpret_cast<const uint16_t *>(head + q8_chunk<HD>(r, lane >> 3) + (lane & 7) * 2);
+}
+
+}  // namespace leap

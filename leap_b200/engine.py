@@ -13,7 +13,8 @@ import ctypes
 
 import numpy as np
 
-from ._native import LeapError, ModelConfigC, check, lib
+from ._native import LEAP_KV_F32, LeapError, ModelConfigC, check, lib
+from .attention import kv_kind
 from .modelfile import ModelConfig
 
 FLAG_NO_REPLY = 0    # src/inference/Transformer.h:45
@@ -44,18 +45,19 @@ class Transformer:
     # -- construction ---------------------------------------------------------
     @staticmethod
     def create(checkpoint_path: str, device: int = 0, rope_theta: float = 0.0,
-               layer_range=None, max_chunk: int = 512) -> "Transformer":
-        """Transformer::create (src/inference/TransformerFactory.cpp:59)."""
+               layer_range=None, max_chunk: int = 512, kv: str = "f32") -> "Transformer":
+        """Transformer::create (src/inference/TransformerFactory.cpp:59).
+        ``kv``: how cached rows are kept (``"f32"`` or ``"q8"``, 8 bits)."""
         lb, le = layer_range if layer_range is not None else (0, -1)
         h = ctypes.c_void_p()
         check(lib().leap_engine_open(checkpoint_path.encode(), device, lb, le,
                                      ctypes.c_float(rope_theta), max_chunk, ctypes.byref(h)))
-        return Transformer(h)
+        return Transformer(h)._with_kv(kv)
 
     @staticmethod
     def synthetic(config: ModelConfig, quantized: bool, seed: int = 0, group_size: int = 64,
                   device: int = 0, rope_theta: float = 0.0, layer_range=None,
-                  max_chunk: int = 512) -> "Transformer":
+                  max_chunk: int = 512, kv: str = "f32") -> "Transformer":
         """N(0, 0.02) weights generated on the device (no file)."""
         lb, le = layer_range if layer_range is not None else (0, -1)
         c = ModelConfigC(*config.as_tuple(), int(quantized), group_size if quantized else 0, 1)
@@ -63,7 +65,18 @@ class Transformer:
         check(lib().leap_engine_synthetic(ctypes.byref(c), seed, device, lb, le,
                                           ctypes.c_float(rope_theta), max_chunk,
                                           ctypes.byref(h)))
-        return Transformer(h)
+        return Transformer(h)._with_kv(kv)
+
+    def _with_kv(self, kv: str) -> "Transformer":
+        if kv_kind(kv) != LEAP_KV_F32:
+            self.set_kv(kv)
+        return self
+
+    def set_kv(self, kv: str) -> None:
+        """Replace the KV cache by an empty one whose rows are kept as ``kv``
+        says: ``"f32"``, or ``"q8"`` (a byte a value, about a quarter of the
+        memory and of the bytes a decode step reads)."""
+        check(lib().leap_engine_set_kv(self.handle, kv_kind(kv)))
 
     def close(self) -> None:
         if getattr(self, "_h", None):
