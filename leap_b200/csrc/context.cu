@@ -98,6 +98,8 @@ int check_device_error(leap_ctx *c) {
     for (int i = 0; i < 2; ++i)
         if (c->counters[i])
             cudaMemset(c->counters[i], 0, sizeof(unsigned) * kMaxSeqPerLaunch * c->n_kv);
+    if (c->q8_counters)
+        cudaMemset(c->q8_counters, 0, sizeof(unsigned) * kMaxSeqPerLaunch * c->n_kv);
     if (err == kDevErrBadToken)
         set_error("a device-side token id was outside [0, vocab_size)");
     else
@@ -503,7 +505,9 @@ static int decode_launch(leap_ctx *c, int layer, const leap::DecodeSeq &tab, con
         s.tok0[i] = i;
     }
     s.tok0[tab.n_seq] = tab.n_seq;
-    return leap::q8_attend(c, layer, s, nullptr, q, k_new, v_new, out);
+    const int st = leap::q8_attend(c, layer, s, nullptr, q, k_new, v_new, out);
+    c->last_written_layer = layer;
+    return st;
 }
 
 int leap_attn_decode(leap_ctx *c, int layer, int pos, const float *q, const float *k_new,

@@ -33,6 +33,10 @@ struct leap_ctx {
     float *ks8 = nullptr, *vs8 = nullptr;
     size_t head_rows = 0, layer_rows = 0, slot_rows = 0;
     float *d_rows = nullptr;  // FP32 rows on their way from or to host memory
+    // its split-KV scratch: partials of up to 8 rows, and tickets
+    float *q8_part_o = nullptr, *q8_part_ml = nullptr;  // [q8_parts][8][hd], [q8_parts][8][2]
+    unsigned *q8_counters = nullptr;                    // [kMaxSeqPerLaunch][n_kv]
+    int q8_parts = 0;
 
     // RoPE table [max_seq][hd/2]
     float *rope_cos = nullptr, *rope_sin = nullptr;
@@ -161,6 +165,14 @@ struct Q8Tree {
     int8_t parent[kMaxNodesPerLaunch];
 };
 
+// Splits of the sequences' cached rows: `chunk` rows each, sequence i's are
+// split0[i] .. split0[i+1]-1 (none for a sequence without new tokens).
+struct Q8Splits {
+    int chunk;
+    int split0[kMaxSeqPerLaunch + 1];
+};
+constexpr int kQ8Rows = 8;  // query rows (tokens x heads of a group) of the rows kernel
+
 // One layer of the cache as kernels see it.
 struct Q8Layer {
     uint8_t *k, *v;    // codes of (slot 0, this layer, kv head 0)
@@ -182,6 +194,9 @@ int q8_append(leap_ctx *c, int layer, const Q8Seqs &tab, const Q8Tree *tree, con
 int kv_read_packed(leap_ctx *c, int layer, const Q8Seqs &tab, float *k, float *v);
 // Move rows pos + node[j] to pos + j (j counted from each sequence's first).
 int kv_keep(leap_ctx *c, const Q8Seqs &tab, const Q8Tree &nodes);
+int q8_rows_parts(const leap_ctx *c);
+int q8_rows_attend(leap_ctx *c, int layer, const Q8Seqs &tab, const Q8Tree *tree, const float *q,
+                   const float *k, const float *v, float *out);
 // Append and attend: causal, or a tree of each sequence's tokens.
 int q8_attend(leap_ctx *c, int layer, const Q8Seqs &tab, const Q8Tree *tree, const float *q,
               const float *k, const float *v, float *out);

@@ -28,7 +28,8 @@ template <int HD, int MODE>
 __global__ void __launch_bounds__(32 * kWarps)
 q8_append_kernel(const float *__restrict__ k, const float *__restrict__ v, const Q8Layer L,
                  const float *__restrict__ rope_cos, const float *__restrict__ rope_sin,
-                 const __grid_constant__ Q8Seqs tab, const __grid_constant__ Q8Tree tree) {
+                 const __grid_constant__ Q8Seqs tab,
+                 const __grid_constant__ Q8See<MODE == kTree> see) {
     constexpr int E = HD / 32;
     grid_launch_dependents();  // what follows waits for this grid before it reads
     const int lane = threadIdx.x & 31;
@@ -49,12 +50,7 @@ q8_append_kernel(const float *__restrict__ k, const float *__restrict__ v, const
         y[e] = reinterpret_cast<const float *>(&vx)[e];
     }
     if (MODE != kRaw) {
-        int at = row;
-        if (MODE == kTree) {
-            at = tab.pos[seq];
-            const int8_t *parent = tree.parent + tab.tok0[seq];
-            for (int p = parent[i]; p >= 0; p = parent[p]) ++at;  // parents come before children
-        }
+        const int at = tab.pos[seq] + see.depth(tab.tok0[seq], i);
         const float *rc = rope_cos + size_t(at) * (HD / 2) + lane * (E / 2);
         const float *rs = rope_sin + size_t(at) * (HD / 2) + lane * (E / 2);
 #pragma unroll
@@ -172,13 +168,12 @@ f32_keep_kernel(float *kc, float *vc, size_t head_stride, size_t layer_stride, s
 }
 
 template <int HD, int MODE>
-int launch_append(leap_ctx *c, int layer, const Q8Seqs &tab, const Q8Tree *tree, const float *k,
-                  const float *v) {
-    static const Q8Tree none = {};
+int launch_append(leap_ctx *c, int layer, const Q8Seqs &tab, const Q8See<MODE == kTree> &see,
+                  const float *k, const float *v) {
     const int items = tab.tok0[tab.n_seq] * c->n_kv;
     if (items == 0) return LEAP_OK;
     q8_append_kernel<HD, MODE><<<(items + kWarps - 1) / kWarps, 32 * kWarps, 0, c->stream>>>(
-        k, v, q8_layer(c, layer), c->rope_cos, c->rope_sin, tab, tree ? *tree : none);
+        k, v, q8_layer(c, layer), c->rope_cos, c->rope_sin, tab, see);
     return cuda_status(cudaGetLastError(), "q8_append_kernel launch");
 }
 
@@ -204,8 +199,8 @@ Q8Seqs one_run(int slot, int pos0, int n) {
 }
 
 int write_rows(leap_ctx *c, int layer, const Q8Seqs &tab, const float *k, const float *v) {
-    return c->hd == 128 ? launch_append<128, kRaw>(c, layer, tab, nullptr, k, v)
-                        : launch_append<64, kRaw>(c, layer, tab, nullptr, k, v);
+    return c->hd == 128 ? launch_append<128, kRaw>(c, layer, tab, {}, k, v)
+                        : launch_append<64, kRaw>(c, layer, tab, {}, k, v);
 }
 
 }  // namespace
@@ -227,8 +222,15 @@ int q8_create(leap_ctx *c) {
     if (e == cudaSuccess) e = cudaMalloc(&c->ks8, rows * sizeof(float));
     if (e == cudaSuccess) e = cudaMalloc(&c->vs8, rows * sizeof(float));
     if (e == cudaSuccess) e = cudaMalloc(&c->d_rows, stage);
+    c->q8_parts = q8_rows_parts(c);
+    const size_t part = size_t(c->q8_parts) * kQ8Rows * sizeof(float);
+    const size_t cnt = size_t(kMaxSeqPerLaunch) * c->n_kv * sizeof(unsigned);
+    if (e == cudaSuccess) e = cudaMalloc(&c->q8_part_o, part * c->hd);
+    if (e == cudaSuccess) e = cudaMalloc(&c->q8_part_ml, part * 2);
+    if (e == cudaSuccess) e = cudaMalloc(&c->q8_counters, cnt);
+    if (e == cudaSuccess) e = cudaMemset(c->q8_counters, 0, cnt);
     if (e != cudaSuccess) return cuda_status(e, "cudaMalloc(8-bit cache)");
-    c->device_bytes += 2 * rows * (c->hd + sizeof(float)) + stage;
+    c->device_bytes += 2 * rows * (c->hd + sizeof(float)) + stage + part * (c->hd + 2) + cnt;
     return q8_clear(c);
 }
 
@@ -238,6 +240,9 @@ void q8_free(leap_ctx *c) {
     cudaFree(c->ks8);
     cudaFree(c->vs8);
     cudaFree(c->d_rows);
+    cudaFree(c->q8_part_o);
+    cudaFree(c->q8_part_ml);
+    cudaFree(c->q8_counters);
 }
 
 int q8_clear(leap_ctx *c) {
@@ -286,10 +291,10 @@ int q8_read(leap_ctx *c, int slot, int layer, int pos0, int n, float *k, float *
 int q8_append(leap_ctx *c, int layer, const Q8Seqs &tab, const Q8Tree *tree, const float *k,
               const float *v) {
     if (c->hd == 128)
-        return tree ? launch_append<128, kTree>(c, layer, tab, tree, k, v)
-                    : launch_append<128, kCausal>(c, layer, tab, nullptr, k, v);
-    return tree ? launch_append<64, kTree>(c, layer, tab, tree, k, v)
-                : launch_append<64, kCausal>(c, layer, tab, nullptr, k, v);
+        return tree ? launch_append<128, kTree>(c, layer, tab, q8_see(*tree), k, v)
+                    : launch_append<128, kCausal>(c, layer, tab, {}, k, v);
+    return tree ? launch_append<64, kTree>(c, layer, tab, q8_see(*tree), k, v)
+                : launch_append<64, kCausal>(c, layer, tab, {}, k, v);
 }
 
 int kv_read_packed(leap_ctx *c, int layer, const Q8Seqs &tab, float *k, float *v) {

@@ -43,6 +43,34 @@ __device__ __forceinline__ int q8_seq_of(const Q8Seqs &tab, int t) {
     return lo;
 }
 
+// How the tokens of a run see one another.  Causal: token i sees 0..i, at
+// position pos + i.  Tree: i sees itself and its ancestors, at pos + depth.
+template <bool TREE>
+struct Q8See;
+template <>
+struct Q8See<false> {
+    __device__ __forceinline__ int depth(int, int i) const { return i; }
+    __device__ __forceinline__ bool sees(int, int i, int j) const { return j <= i; }
+};
+template <>
+struct Q8See<true> {
+    Q8Tree tree;
+    // t0: the sequence's first packed token.  Parents come before children.
+    __device__ __forceinline__ int depth(int t0, int i) const {
+        int d = 0;
+        for (int p = tree.parent[t0 + i]; p >= 0; p = tree.parent[t0 + p]) ++d;
+        return d;
+    }
+    __device__ __forceinline__ bool sees(int t0, int i, int j) const {
+        while (i > j) i = tree.parent[t0 + i];
+        return i == j;
+    }
+};
+inline const Q8See<true> &q8_see(const Q8Tree &tree) {
+    static_assert(sizeof(Q8See<true>) == sizeof(Q8Tree), "one is the other");
+    return reinterpret_cast<const Q8See<true> &>(tree);
+}
+
 // The code nearest to x / s (ties to even), `s` normal and inv near 1 / s:
 // the rounded product is at most one off, and the residual x - q*s, exact in
 // one fused multiply-add, tells on which side of the half x lies.
