@@ -234,7 +234,7 @@ q8_rows_kernel(const RowsArgs a, const __grid_constant__ Q8Seqs tab,
     fence_mbar_init();
     __syncwarp();
     auto request = [&](int i) {
-        // whole groups of 8 rows (the cache has room for 64 at a time): rows
+        // whole groups of 8 rows (the cache has room for 128 at a time): rows
         // past the end are read as they are and masked
         const int first = row0 + (warp + i * W) * kTile;
         const int n = min(kTile, (row1 - first + 7) & ~7);
@@ -511,7 +511,7 @@ constexpr int kMinChunk = 128, kMaxChunk = 2048;
 
 int q8_rows_parts(const leap_ctx *c) {
     const long nb = c->max_batch < kMaxSeqPerLaunch ? c->max_batch : kMaxSeqPerLaunch;
-    return int(nb * c->n_kv * (c->max_seq_pad / kMaxChunk + 2) + 2 * c->num_sms);
+    return int(nb * c->n_kv * (c->max_seq / kMaxChunk + 2) + 2 * c->num_sms);
 }
 
 static void plan_rows(const leap_ctx *c, const Q8Seqs &tab, Q8Splits &plan) {

@@ -1,0 +1,763 @@
+// attn_q8_tc.cu — attention of many query rows for each kv head (packed
+// prompts, drafted trees) over the 8-bit KV cache, on tcgen05 tensor cores.
+//
+//   out = softmax(rope(q) . (c_k s_k) / sqrt(hd)) . (c_v s_v)
+//
+// The append kernel (kv_q8.cu) has stored the run's own rows; this kernel reads
+// cached rows only.  A block takes 128 query rows (row r is token r / G of its
+// tile, head r % G of the kv head's group) and a range of key tiles of 128.
+//
+// Arithmetic: codes are exact in FP16.  Queries (scaled by a power of two for
+// each row) and weights p*s_v (by one for each tile) are split into two FP16,
+// hi + lo, 22 bits: two FP16 products in place of one give FP32-like results,
+// and are what bounds the kernel (twice the FLOPs of one FP16 product; 32
+// tcgen05.mma of 128x128x16 a tile, about 2048 cycles).  Tensor-core sums are
+// truncated and would drift over a long context, so O is summed from zero for
+// every tile and joins FP32 registers by ordinary multiply-adds, with the
+// running maximum's correction: nothing is rescaled in TMEM.
+//
+// Roles (16 warps; registers moved to where O lives by setmaxnreg, 200 + 200 +
+// 72 + 40 = 4 x 128):
+//   warps 0-3, 4-7   two softmax groups; group b takes tiles b, b+2, ...: S(j)
+//                    from TMEM, p, hi/lo back over S in place, then O(j) into
+//                    its registers.  Each keeps its own maximum, sum and output;
+//                    the two are joined at the end.  While one waits for its
+//                    PV product the other works.
+//   warps 8-11       codes -> FP16 operand tiles (128-byte swizzle; V is used
+//                    N-major, so nothing is transposed), a tile ahead in
+//                    registers, and the tile's scales.
+//   warp 12          issues S(j) = Q K^T and O(j) = P V, whichever is ready.
+// TMEM: S/P and O of either group (2 x (128 + HD) columns).  Shared memory:
+// Q hi/lo, two buffers each of K and V.
+// Long ranges are split over blocks when a launch has few tiles; partials are
+// joined by a second kernel.
+#include <algorithm>
+#include <atomic>
+
+#include "q8.cuh"
+#include "tc.cuh"
+
+namespace leap {
+namespace {
+
+constexpr int kBM = 128;        // query rows of a block = TMEM lanes
+constexpr int kBN = 128;        // keys of a tile
+constexpr int kThreads = 512;
+constexpr int kLaunchRegs = 65536 / kThreads;
+constexpr int kRegsSoftmax = 200, kRegsConvert = 72, kRegsIssue = 40;  // of each group of 4 warps
+static_assert(2 * kRegsSoftmax + kRegsConvert + kRegsIssue == 4 * kLaunchRegs, "register split");
+constexpr int kSlots = 4;       // tiles whose scales are held
+
+template <int HD>
+struct Tc {
+    static constexpr uint32_t kOp = kBN * HD * 2;           // one operand tile
+    static constexpr uint32_t kChunk = 128 * 128;           // 64 dims of 128 rows
+    static constexpr uint32_t kQ = 0, kK = 2 * kOp, kV = 4 * kOp;
+    static constexpr size_t kSmem = 6 * size_t(kOp) + 1024;
+    static constexpr uint32_t kCols = 512;                  // TMEM columns (a power of two)
+    static constexpr uint32_t kColS(int b) { return b * 128; }
+    static constexpr uint32_t kColO(int b) { return 256 + b * HD; }
+};
+
+struct TcArgs {
+    const float *q;
+    float *out;
+    Q8Layer L;
+    const float *rope_cos, *rope_sin;
+    float *part_o, *part_ml;  // [parts][HD/4][128] float4, [parts][128][2]
+    int *err;
+    float scale_log2;
+};
+
+struct TcBars {
+    uint64_t q_ready;    // Q in shared memory (8 softmax warps)
+    uint64_t k_full[2], v_full[2];  // operand tile in place (4 converter warps)
+    uint64_t sc_full[kSlots];       // scales of a tile in place (4 converter warps)
+    uint64_t s_full[2];  // S(j) done: K buffer free (commit)
+    uint64_t p_full[2];  // P(j) in TMEM (4 softmax warps)
+    uint64_t o_full[2];  // O(j) done: V buffer and S/P columns free (commit)
+};
+
+__device__ __forceinline__ uint32_t par(int j) { return uint32_t(j >> 1) & 1u; }
+
+// Which (sequence, query tile, split, kv head) a block has.
+struct Item {
+    int seq, qt, split, h, part;
+};
+__device__ __forceinline__ Item item_of(const Q8TcPlan &plan, int n_kv, int block) {
+    Item it;
+    const int x = block / n_kv;
+    it.h = block - x * n_kv;
+    int lo = 0, hi = plan.n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (plan.item0[mid] <= x) lo = mid; else hi = mid - 1;
+    }
+    it.seq = plan.seq[lo];
+    const int i = x - plan.item0[lo];
+    it.split = i % plan.nsplit[lo];
+    it.qt = plan.n_qt[lo] - 1 - i / plan.nsplit[lo];  // the longest first
+    it.part = plan.nsplit[lo] > 1 ? (plan.part0[lo] + i) * n_kv + it.h : -1;
+    return it;
+}
+
+// Eight codes as FP16 values (a 16-byte granule).
+__device__ __forceinline__ uint4 expand(uint32_t a, uint32_t b) {
+    auto two = [](uint32_t x, uint32_t sel) {
+        const uint32_t y = __byte_perm(x, 0x64646464u, sel);
+        const __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&y), __float2half2_rn(1152.f));
+        return *reinterpret_cast<const uint32_t *>(&h);
+    };
+    return make_uint4(two(a, 0x5140), two(a, 0x5342), two(b, 0x5140), two(b, 0x5342));
+}
+
+template <int N>
+__device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+template <int HD, int G, bool TREE>
+__global__ void __launch_bounds__(kThreads, 1)
+q8_tc_kernel(const TcArgs a, const __grid_constant__ Q8Seqs tab, const __grid_constant__ Q8TcPlan plan,
+             const __grid_constant__ Q8See<TREE> see) {
+    using C = Tc<HD>;
+    constexpr int BT = kBM / G;  // tokens of a block
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ TcBars bars;
+    __shared__ __align__(16) float s_ks[kSlots][kBN], s_vs[kSlots][kBN];
+    __shared__ float s_vdown[kSlots], s_fac[kBM], s_m[kBM], s_l[kBM];
+    __shared__ int8_t s_parent[TREE ? kMaxTreeNodes : 1];
+    __shared__ uint32_t s_anc[TREE ? 4 : 1][kBM];  // TREE: what each row sees of the run
+    __shared__ uint32_t tmem_sh;
+    __shared__ int s_fail;
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    unsigned char *base = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
+    const uint32_t sbase = smem_addr(base);
+
+    const Item it = item_of(plan, a.L.n_kv, blockIdx.x);
+    const int seq = it.seq, h = it.h;
+    const int pos = tab.pos[seq], tok0 = tab.tok0[seq], n_new = tab.tok0[seq + 1] - tok0;
+    const int t0 = it.qt * BT;                       // first token of the tile, within the run
+    const int t_end = min(t0 + BT, n_new);
+    const int kv_end = TREE ? pos + n_new : pos + t_end;
+    const int n_all = (kv_end + kBN - 1) / kBN;
+    const int j0 = it.split * plan.chunk;
+    const int n_kt = max(min(n_all - j0, plan.chunk), 0);  // tiles j0 .. j0 + n_kt - 1
+
+    if (tid == 0) {
+        mbar_init(&bars.q_ready, 8);
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&bars.k_full[b], 4);
+            mbar_init(&bars.v_full[b], 4);
+            mbar_init(&bars.s_full[b], 1);
+            mbar_init(&bars.p_full[b], 4);
+            mbar_init(&bars.o_full[b], 1);
+        }
+        for (int i = 0; i < kSlots; ++i) mbar_init(&bars.sc_full[i], 4);
+        s_fail = 0;
+        fence_mbar_init();
+    }
+    if (warp == 12) {
+        tc::alloc(&tmem_sh, C::kCols);
+        tc::relinquish();
+    }
+    if constexpr (TREE)
+        if (tid < n_new) s_parent[tid] = see.tree.parent[tok0 + tid];
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    const uint32_t tmem = tmem_sh;
+
+    if (warp < 8) {
+        // ================= softmax groups =====================================
+        regs_up<kRegsSoftmax>();
+        const int b = warp >> 2;             // group
+        const int row = tid & 127;           // TMEM lane
+        const uint32_t lane_off = uint32_t((warp & 3) * 32) << 16;
+        // Q was written before the append kernel began, so it needs no wait
+        {
+            constexpr int E = HD / 32, U = 4;
+            for (int r0 = warp; r0 < kBM; r0 += 8 * U) {
+                float x[U][E];
+                int at[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int r = r0 + 8 * u, t = t0 + r / G;
+                    at[u] = -1;
+                    if (t < t_end) {
+                        at[u] = pos + t;
+                        if (TREE) {
+                            at[u] = pos;
+                            for (int p = s_parent[t]; p >= 0; p = s_parent[p]) ++at[u];
+                        }
+                        const float *src = a.q + (size_t(tok0 + t) * a.L.n_kv * G + h * G + r % G) * HD + E * lane;
+#pragma unroll
+                        for (int e = 0; e < E; ++e) x[u][e] = src[e];
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < E; ++e) x[u][e] = 0.f;
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int r = r0 + 8 * u;
+                    float top = 0.f;
+#pragma unroll
+                    for (int e = 0; e < E; e += 2) {
+                        if (at[u] >= 0) {
+                            const size_t c = size_t(at[u]) * (HD / 2) + (E * lane + e) / 2;
+                            const float2 z = rope_pair(x[u][e], x[u][e + 1], a.rope_cos[c], a.rope_sin[c]);
+                            x[u][e] = z.x;
+                            x[u][e + 1] = z.y;
+                        }
+                        top = fmaxf(top, fmaxf(fabsf(x[u][e]), fabsf(x[u][e + 1])));
+                    }
+                    // largest value to [2^14, 2^15); an infinite or NaN query gives NaN
+                    const int ex = min(max(int(__reduce_max_sync(0xffffffffu, __float_as_uint(top)) >> 23), 15), 254);
+                    const float up = __uint_as_float(uint32_t(268 - ex) << 23);
+                    const uint32_t off = tc::sw128_offset_b16(r, E * lane, kBM);
+#pragma unroll
+                    for (int e = 0; e < E; e += 2) {
+                        const float y0 = x[u][e] * up, y1 = x[u][e + 1] * up;
+                        const __half2 hi = __floats2half2_rn(y0, y1);
+                        const float2 back = __half22float2(hi);
+                        *reinterpret_cast<__half2 *>(base + C::kQ + off + 2 * e) = hi;
+                        *reinterpret_cast<__half2 *>(base + C::kQ + C::kOp + off + 2 * e) =
+                            __floats2half2_rn(y0 - back.x, y1 - back.y);
+                    }
+                    if (lane == 0) s_fac[r] = __uint_as_float(uint32_t(ex - 14) << 23) * a.scale_log2;
+                }
+            }
+        }
+        fence_proxy_async_smem();  // Q -> visible to the tensor core
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.q_ready);
+        bool ok = __all_sync(0xffffffffu, mbar_wait(&bars.q_ready, 0));  // s_fac of every row
+
+        // What this row sees: keys below `lim`, or (TREE) keys below pos and
+        // those of the run whose bit is set (itself and its ancestors).
+        const int tok = t0 + row / G;
+        const int lim = pos + min(tok, t_end - 1) + 1;
+        if (TREE && b == 0) {
+            uint32_t anc[4] = {0u, 0u, 0u, 0u};
+            for (int p = min(tok, t_end - 1); p >= 0; p = s_parent[p]) {
+#pragma unroll
+                for (int w = 0; w < 4; ++w)
+                    if ((p >> 5) == w) anc[w] |= 1u << (p & 31);
+            }
+#pragma unroll
+            for (int w = 0; w < 4; ++w) s_anc[w][row] = anc[w];
+        }
+        if (TREE) asm volatile("bar.sync 1, 256;" ::: "memory");
+        // bit i: whether key k0 + i is seen
+        auto seen = [&](int k0) -> uint32_t {
+            if (!TREE) {
+                const int n = lim - k0;
+                return n >= 32 ? ~0u : (n <= 0 ? 0u : (1u << n) - 1u);
+            }
+            const int rel = k0 - pos, w = rel >> 5;  // bits below 0 are all ones, from 128 on zeros
+            const uint32_t lo = w < 0 ? ~0u : (w > 3 ? 0u : s_anc[w][row]);
+            const uint32_t hi = w < -1 ? ~0u : (w > 2 ? 0u : s_anc[w + 1][row]);
+            return __funnelshift_r(lo, hi, rel & 31);
+        };
+
+        const float fac = s_fac[row];
+        float m = -INFINITY, l = 0.f;
+        float o[HD];
+#pragma unroll
+        for (int i = 0; i < HD; ++i) o[i] = 0.f;
+
+        for (int j = b; j < n_kt && ok; j += 2) {
+            ok = mbar_wait(&bars.sc_full[j & (kSlots - 1)], uint32_t(j / kSlots) & 1u) &&
+                 mbar_wait(&bars.s_full[b], par(j));
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc::fence_after_sync();
+            const int slot = j & (kSlots - 1);
+            const int k0 = (j0 + j) * kBN;
+            const uint32_t scol = tmem + lane_off + C::kColS(b);
+            const float4 *ks = reinterpret_cast<const float4 *>(s_ks[slot]);
+            const float4 *vs = reinterpret_cast<const float4 *>(s_vs[slot]);
+            const bool full = __all_sync(0xffffffffu, (TREE ? pos : lim) >= k0 + kBN);
+            // the largest score (in units of 1/fac)
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+                float s[32];
+                tc::ld32(scol + 32 * c, s);
+                tc::wait_ld();
+                const uint32_t vis = full ? ~0u : seen(k0 + 32 * c);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float4 f = ks[8 * c + i];
+                    const float2 x = __fmul2_rn(make_float2(s[4 * i], s[4 * i + 1]), make_float2(f.x, f.y));
+                    const float2 y = __fmul2_rn(make_float2(s[4 * i + 2], s[4 * i + 3]), make_float2(f.z, f.w));
+                    if (full) {
+                        mx[0] = fmaxf(mx[0], x.x);
+                        mx[1] = fmaxf(mx[1], x.y);
+                        mx[2] = fmaxf(mx[2], y.x);
+                        mx[3] = fmaxf(mx[3], y.y);
+                    } else {
+                        if (vis >> (4 * i) & 1) mx[0] = fmaxf(mx[0], x.x);
+                        if (vis >> (4 * i + 1) & 1) mx[1] = fmaxf(mx[1], x.y);
+                        if (vis >> (4 * i + 2) & 1) mx[2] = fmaxf(mx[2], y.x);
+                        if (vis >> (4 * i + 3) & 1) mx[3] = fmaxf(mx[3], y.y);
+                    }
+                }
+            }
+            const float mn = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * fac);
+            const float ref = mn == -INFINITY ? 0.f : mn;  // nothing seen so far
+            const float alpha = fast_exp2(m - ref);
+            m = mn;
+            const float2 fac2 = make_float2(fac, fac), nref2 = make_float2(-ref, -ref);
+            float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll 1
+            for (int c = 0; c < kBN / 16; ++c) {  // 16 keys: one step of the PV product
+                float s[16];
+                tc::ld16(scol + 16 * c, s);
+                tc::wait_ld();
+                const uint32_t vis = full ? ~0u : seen(k0 + 16 * c);
+                uint32_t hl[16];  // 8 words hi, 8 words lo: over the scores they come from
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float2 f = reinterpret_cast<const float2 *>(ks)[8 * c + i];
+                    const float2 g = reinterpret_cast<const float2 *>(vs)[8 * c + i];
+                    const float2 e = __ffma2_rn(__fmul2_rn(make_float2(s[2 * i], s[2 * i + 1]), f), fac2, nref2);
+                    float2 p = make_float2(fast_exp2(e.x), fast_exp2(e.y));
+                    float2 w = __fmul2_rn(p, g);
+                    if (!full) {  // what is not seen takes no part, whatever its scales
+                        if (!(vis >> (2 * i) & 1)) p.x = w.x = 0.f;
+                        if (!(vis >> (2 * i + 1) & 1)) p.y = w.y = 0.f;
+                    }
+                    sum[i & 1] = __fadd2_rn(sum[i & 1], p);
+                    const __half2 hi = __floats2half2_rn(w.x, w.y);
+                    const float2 back = __half22float2(hi);
+                    const float2 r = __fadd2_rn(w, make_float2(-back.x, -back.y));
+                    const __half2 lo = __floats2half2_rn(r.x, r.y);
+                    hl[i] = *reinterpret_cast<const uint32_t *>(&hi);
+                    hl[8 + i] = *reinterpret_cast<const uint32_t *>(&lo);
+                }
+                tc::st16u(scol + 16 * c, hl);
+            }
+            l = l * alpha + ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
+            const float vdown = s_vdown[slot];
+            tc::wait_st();
+            tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars.p_full[b]);
+            ok = __all_sync(0xffffffffu, mbar_wait(&bars.o_full[b], par(j)));
+            if (!ok) break;
+            tc::fence_after_sync();
+            const float2 al2 = make_float2(alpha, alpha), vd2 = make_float2(vdown, vdown);
+#pragma unroll
+            for (int c = 0; c < HD / 32; ++c) {
+                float x[32];
+                tc::ld32(tmem + lane_off + C::kColO(b) + 32 * c, x);
+                tc::wait_ld();
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                    const float2 z = __ffma2_rn(make_float2(x[i], x[i + 1]), vd2,
+                                                __fmul2_rn(make_float2(o[32 * c + i], o[32 * c + i + 1]), al2));
+                    o[32 * c + i] = z.x;
+                    o[32 * c + i + 1] = z.y;
+                }
+            }
+            tc::fence_before_sync();  // O(j) read before PV(j+2), which p_full(j+2) allows
+        }
+        if (!ok && lane == 0) atomicExch(&s_fail, 1);
+        // ---- join the two groups: group 1's state through shared memory ---------
+        // (both groups are past their last tile here, so no buffer is in use;
+        // named barrier 1: the 256 threads of both)
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        float4 *s_o = reinterpret_cast<float4 *>(base + C::kK);  // [HD/4][128]
+        if (b == 1) {
+            s_m[row] = m;
+            s_l[row] = l;
+#pragma unroll
+            for (int i = 0; i < HD / 4; ++i)
+                s_o[i * kBM + row] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        }
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (b == 0 && !*reinterpret_cast<volatile int *>(&s_fail)) {
+            const float m1 = s_m[row], mm = fmaxf(m, m1);
+            const float e0 = m == -INFINITY ? 0.f : fast_exp2(m - mm);
+            const float e1 = m1 == -INFINITY ? 0.f : fast_exp2(m1 - mm);
+            const float sum = l * e0 + s_l[row] * e1;
+            if (it.part < 0) {
+                const float inv = 1.f / sum;
+                float *dst = a.out + (size_t(tok0 + tok) * a.L.n_kv * G + h * G + row % G) * HD;
+#pragma unroll
+                for (int i = 0; i < HD / 4; ++i) {
+                    const float4 x = s_o[i * kBM + row];
+                    float4 v;
+                    v.x = (o[4 * i] * e0 + x.x * e1) * inv;
+                    v.y = (o[4 * i + 1] * e0 + x.y * e1) * inv;
+                    v.z = (o[4 * i + 2] * e0 + x.z * e1) * inv;
+                    v.w = (o[4 * i + 3] * e0 + x.w * e1) * inv;
+                    if (tok < t_end) *reinterpret_cast<float4 *>(dst + 4 * i) = v;
+                }
+            } else if (tok < t_end) {
+                float4 *po = reinterpret_cast<float4 *>(a.part_o) + size_t(it.part) * (HD / 4) * kBM + row;
+#pragma unroll
+                for (int i = 0; i < HD / 4; ++i) {
+                    const float4 x = s_o[i * kBM + row];
+                    po[i * kBM] = make_float4(o[4 * i] * e0 + x.x * e1, o[4 * i + 1] * e0 + x.y * e1,
+                                              o[4 * i + 2] * e0 + x.z * e1, o[4 * i + 3] * e0 + x.w * e1);
+                }
+                reinterpret_cast<float2 *>(a.part_ml)[size_t(it.part) * kBM + row] = make_float2(mm, sum);
+            }
+        }
+    } else if (warp < 12) {
+        // ================= converters: codes -> FP16 operand tiles =============
+        regs_down<kRegsConvert>();
+        constexpr int N = kBN * HD / 16 / 128;  // 16-byte chunks of a tile a thread takes
+        const int ct = tid - 256;
+        const size_t r0 = tab.slot[seq] * a.L.slot_rows + h * a.L.head_rows;
+        const uint8_t *gk = a.L.k + r0 * HD, *gv = a.L.v + r0 * HD;
+        const float *gks = a.L.ks + r0, *gvs = a.L.vs + r0;
+        grid_dependency_wait();  // the append kernel has stored the run's rows
+        grid_launch_dependents();
+        // Half an operand tile is in flight while the half before it is stored:
+        // K's two halves, V's two, the next tile's K, ... in two register sets.
+        constexpr int N2 = N / 2;
+        uint4 w[2][N2];
+        auto load = [&](const uint8_t *g, int j, int half) {
+            const uint4 *src = reinterpret_cast<const uint4 *>(g + size_t(j0 + j) * kBN * HD) + ct + half * 128 * N2;
+#pragma unroll
+            for (int i = 0; i < N2; ++i) w[half][i] = src[128 * i];
+        };
+        // Chunk ct + 128 i (16 bytes each) of a tile: its line is (ct >> 3) + 16 i,
+        // so its dims and its place in an 8-row swizzle group are the same for
+        // every i.  Chunks 4-7 store their upper half first: eight neighbouring
+        // threads then meet eight different bank groups.
+        int row, ch;
+        if (HD == 128) {
+            row = ct >> 3;
+            ch = (ct & 7) ^ ((((row >> 1) & 3) << 1) ^ ((row & 1) << 2));
+        } else {
+            const int x = (ct & 7) ^ (((ct >> 3) & 3) << 1);
+            row = 2 * (ct >> 3) + (x >> 2);
+            ch = x & 3;
+        }
+        constexpr uint32_t kStep = HD == 128 ? 2048 : 4096;  // 16 or 32 rows on
+        const bool upper = ch & 4;
+        const uint32_t g0 = (ch >> 2) * C::kChunk + (row >> 3) * 1024 + (row & 7) * 128 +
+                            (((2 * (ch & 3) + upper) ^ (row & 7)) << 4);
+        auto store = [&](uint32_t dst, int half) {
+            unsigned char *d0 = base + dst + g0 + half * N2 * kStep, *d1 = base + dst + (g0 ^ 16) + half * N2 * kStep;
+#pragma unroll
+            for (int i = 0; i < N2; ++i) {
+                const uint4 x = w[half][i];
+                *reinterpret_cast<uint4 *>(d0 + i * kStep) = expand(upper ? x.z : x.x, upper ? x.w : x.y);
+                *reinterpret_cast<uint4 *>(d1 + i * kStep) = expand(upper ? x.x : x.z, upper ? x.y : x.w);
+            }
+        };
+        bool ok = true;
+        if (n_kt > 0) {
+            load(gk, 0, 0);
+            load(gk, 0, 1);
+        }
+        for (int j = 0; j < n_kt && ok; ++j) {
+            const int b = j & 1, slot = j & (kSlots - 1);
+            if (j >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&bars.s_full[b], par(j - 2)));
+            if (!ok) break;
+            // Scales (of rows the block may see; the others count as 0).  Slot
+            // j % 4 was last read for tile j - 4: S(j-2) was issued after
+            // PV(j-4), that after the softmax of tile j-4.
+            {
+                const int first = (j0 + j) * kBN, n = kv_end - first;
+                float top = 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int r = 32 * i + lane;
+                    const float x = r < n ? gvs[first + r] : 0.f;
+                    top = fmaxf(top, x < INFINITY ? x : 0.f);
+                }
+                const int e = max(int(__reduce_max_sync(0xffffffffu, __float_as_uint(top)) >> 23), 15);
+                const float vup = __uint_as_float(uint32_t(268 - e) << 23);
+                s_ks[slot][ct] = ct < n ? gks[first + ct] : 0.f;
+                s_vs[slot][ct] = ct < n ? gvs[first + ct] * vup : 0.f;
+                if (ct == 0) s_vdown[slot] = __uint_as_float(uint32_t(e - 14) << 23);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars.sc_full[slot]);
+            }
+            store(C::kK + b * C::kOp, 0);
+            load(gv, j, 0);
+            store(C::kK + b * C::kOp, 1);
+            load(gv, j, 1);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars.k_full[b]);
+            if (j >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&bars.o_full[b], par(j - 2)));
+            if (!ok) break;
+            store(C::kV + b * C::kOp, 0);
+            if (j + 1 < n_kt) load(gk, j + 1, 0);
+            store(C::kV + b * C::kOp, 1);
+            if (j + 1 < n_kt) load(gk, j + 1, 1);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars.v_full[b]);
+        }
+        if (!ok && lane == 0) atomicExch(&s_fail, 1);
+    } else {
+        regs_down<kRegsIssue>();
+        if (warp == 12) {
+            // ================= MMA issuer ======================================
+            const bool leader = tc::elect_one_sync();
+            constexpr uint32_t idesc_s = tc::idesc_f16(kBM, kBN, false);
+            constexpr uint32_t idesc_o = tc::idesc_f16(kBM, HD, true);
+            const uint64_t dq = tc::sw128_kmajor_desc(sbase + C::kQ);
+            const uint64_t dk = tc::sw128_kmajor_desc(sbase + C::kK);
+            const uint64_t dv = tc::sw128_nmajor_desc(sbase + C::kV, C::kChunk);
+            int s_issued = 0, pv_issued = 0;
+            bool ok = __all_sync(0xffffffffu, mbar_wait(&bars.q_ready, 0));
+            unsigned long long t_idle = global_ns();
+            uint32_t idle = 0;
+            while (ok && pv_issued < n_kt) {
+                bool progress = false;
+                if (s_issued < n_kt && s_issued <= pv_issued + 1) {
+                    const int j = s_issued, b = j & 1;
+                    bool ready = mbar_test(&bars.k_full[b], par(j));
+                    if (ready && j >= 2) ready = mbar_test(&bars.o_full[b], par(j - 2));
+                    if (__all_sync(0xffffffffu, ready)) {
+                        tc::fence_after_sync();
+                        if (leader) {  // S(j) = (Q hi + Q lo) K^T
+                            const uint64_t k = dk + uint64_t(b) * (C::kOp >> 4);
+#pragma unroll 1
+                            for (int u = 0; u < 2; ++u)
+#pragma unroll 1
+                                for (int kk = 0; kk < HD / 16; ++kk) {
+                                    const uint64_t off = ((kk >> 2) * C::kChunk + (kk & 3) * 32) >> 4;
+                                    tc::mma_f16_ss(tmem + C::kColS(b), dq + u * (C::kOp >> 4) + off, k + off,
+                                                   idesc_s, u + kk > 0 ? 1u : 0u);
+                                }
+                            tc::commit(&bars.s_full[b]);
+                        }
+                        __syncwarp();
+                        ++s_issued;
+                        progress = true;
+                    }
+                }
+                if (pv_issued < s_issued) {
+                    const int j = pv_issued, b = j & 1;
+                    if (__all_sync(0xffffffffu, mbar_test(&bars.p_full[b], par(j)) &&
+                                                    mbar_test(&bars.v_full[b], par(j)))) {
+                        tc::fence_after_sync();
+                        if (leader) {  // O(j) = (P hi + P lo) V, from zero
+                            const uint64_t v = dv + uint64_t(b) * (C::kOp >> 4);
+#pragma unroll 1
+                            for (int kk = 0; kk < kBN / 16; ++kk)
+#pragma unroll 1
+                                for (int u = 0; u < 2; ++u)
+                                    tc::mma_bf16_ts(tmem + C::kColO(b),
+                                                    tmem + C::kColS(b) + 16 * kk + 8 * u,
+                                                    v + uint64_t(kk * 2048 >> 4), idesc_o, u + kk > 0 ? 1u : 0u);
+                            tc::commit(&bars.o_full[b]);
+                        }
+                        __syncwarp();
+                        ++pv_issued;
+                        progress = true;
+                    }
+                }
+                if (progress) {
+                    idle = 0;
+                } else if ((++idle & 255) == 0) {
+                    const unsigned long long t = global_ns();
+                    if (idle == 256) t_idle = t;
+                    else if (t - t_idle > kMaxWaitNs || idle >= kMaxWaitPolls) ok = false;
+                }
+            }
+            if (!ok && leader) atomicExch(&s_fail, 1);
+            // nothing may be in flight when shared memory and TMEM go: wait
+            // (bounded) for the last product of either kind in either buffer
+            for (int b = 0; b < 2; ++b) {
+                const int ls = s_issued - 1 - ((s_issued - 1 - b) & 1);
+                if (ls >= 0) (void)mbar_wait(&bars.s_full[b], par(ls));
+                const int lp = pv_issued - 1 - ((pv_issued - 1 - b) & 1);
+                if (lp >= 0) (void)mbar_wait(&bars.o_full[b], par(lp));
+            }
+        }
+    }
+    tc::fence_before_sync();
+    __syncthreads();
+    if (tid == 0 && s_fail) report_error(a.err, kDevWaitTimeout);
+    if (warp == 12) tc::dealloc(tmem, C::kCols);
+}
+
+// Join the splits: one warp for each query row of a tile that was split.
+template <int HD, int G>
+__global__ void __launch_bounds__(256)
+q8_tc_join_kernel(const TcArgs a, const __grid_constant__ Q8Seqs tab, const __grid_constant__ Q8TcPlan plan) {
+    grid_launch_dependents();
+    grid_dependency_wait();
+    const int lane = threadIdx.x & 31;
+    const int n_kv = a.L.n_kv;
+    // block: 8 rows of a (query tile, kv head); tiles numbered as in the plan
+    const int tile = blockIdx.x / (kBM / 8), row = (blockIdx.x % (kBM / 8)) * 8 + (threadIdx.x >> 5);
+    const int x = tile / n_kv, h = tile - x * n_kv;
+    int lo = 0, hi = plan.n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (plan.tile0[mid] <= x) lo = mid; else hi = mid - 1;
+    }
+    const int ns = plan.nsplit[lo], seq = plan.seq[lo];
+    if (ns == 1) return;
+    const int i = x - plan.tile0[lo], qt = plan.n_qt[lo] - 1 - i;
+    const int tok = qt * (kBM / G) + row / G;
+    const int tok0 = tab.tok0[seq];
+    if (tok >= tab.tok0[seq + 1] - tok0) return;
+    const size_t p0 = size_t(plan.part0[lo] + i * ns) * n_kv + h;  // splits n_kv apart
+    const float2 *ml = reinterpret_cast<const float2 *>(a.part_ml) + p0 * kBM + row;
+    const float4 *po = reinterpret_cast<const float4 *>(a.part_o) + p0 * (HD / 4) * kBM + row;
+    float mx = -INFINITY;
+    for (int s = lane; s < ns; s += 32) mx = fmaxf(mx, ml[size_t(s) * n_kv * kBM].x);
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+    float sum = 0.f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int s = 0; s < ns; ++s) {
+        const float2 y = ml[size_t(s) * n_kv * kBM];
+        const float4 z = lane < HD / 4 ? po[size_t(s) * n_kv * (HD / 4) * kBM + size_t(lane) * kBM]
+                                       : make_float4(0.f, 0.f, 0.f, 0.f);
+        if (y.x == -INFINITY) continue;  // the split had nothing this row sees
+        const float e = fast_exp2(y.x - mx);
+        sum += y.y * e;
+        v.x += z.x * e; v.y += z.y * e; v.z += z.z * e; v.w += z.w * e;
+    }
+    const float inv = 1.f / sum;
+    if (lane < HD / 4)
+        *reinterpret_cast<float4 *>(a.out + (size_t(tok0 + tok) * n_kv * G + h * G + row % G) * HD + 4 * lane) =
+            make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+}
+
+template <int HD, int G, bool TREE>
+int launch_tc(leap_ctx *c, const TcArgs &a, const Q8Seqs &tab, const Q8TcPlan &plan, const Q8See<TREE> &see) {
+    auto fn = q8_tc_kernel<HD, G, TREE>;
+    if (int st = set_kernel_smem(reinterpret_cast<const void *>(fn), Tc<HD>::kSmem, "cudaFuncSetAttribute(q8_tc)"))
+        return st;
+    // The register split adds up to 128 a thread; a build that launches with
+    // fewer would wait for registers that never come.
+    static std::atomic<bool> checked{false};
+    if (!checked.load(std::memory_order_relaxed)) {
+        cudaFuncAttributes fa;
+        if (int st = cuda_status(cudaFuncGetAttributes(&fa, fn), "cudaFuncGetAttributes(q8_tc)")) return st;
+        if (fa.numRegs != kLaunchRegs) {
+            set_error("q8_tc_kernel was built with %d registers a thread, not %d", fa.numRegs, kLaunchRegs);
+            return LEAP_ERR_CUDA;
+        }
+        checked.store(true, std::memory_order_relaxed);
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(unsigned(plan.item0[plan.n]) * c->n_kv);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = Tc<HD>::kSmem;
+    cfg.stream = c->stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;  // it waits before it reads the cache
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int st = cuda_status(cudaLaunchKernelEx(&cfg, fn, a, tab, plan, see), "q8_tc_kernel launch");
+    if (st != LEAP_OK || plan.n_parts == 0) return st;
+    cfg.gridDim = dim3(unsigned(plan.tile0[plan.n]) * c->n_kv * (kBM / 8));
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = 0;
+    return cuda_status(cudaLaunchKernelEx(&cfg, q8_tc_join_kernel<HD, G>, a, tab, plan), "q8_tc_join_kernel launch");
+}
+
+template <int HD, int G>
+int launch_tc_g(leap_ctx *c, const TcArgs &a, const Q8Seqs &tab, const Q8TcPlan &plan, const Q8Tree *tree) {
+    return tree ? launch_tc<HD, G, true>(c, a, tab, plan, q8_see(*tree))
+                : launch_tc<HD, G, false>(c, a, tab, plan, Q8See<false>());
+}
+
+// A block's work apart from its tiles (queries, first loads, output) costs
+// about as much as this many tiles.
+constexpr long kOverhead = 3;
+
+// Sequences longest first, and the tiles of a split.  Blocks are handed to SMs
+// as they fall free, so a launch takes about (all work) / SMs + the longest
+// block; the chunk with the least of that is taken, among those whose partials
+// fit the scratch.
+void plan_tc(const leap_ctx *c, const Q8Seqs &tab, bool tree, Q8TcPlan &plan) {
+    const int bt = kBM / c->group;
+    plan.n = 0;
+    for (int i = 0; i < tab.n_seq; ++i)
+        if (tab.tok0[i + 1] > tab.tok0[i]) plan.seq[plan.n++] = i;
+    auto rows = [&](int i) { return tab.pos[i] + tab.tok0[i + 1] - tab.tok0[i]; };
+    std::sort(plan.seq, plan.seq + plan.n, [&](int x, int y) { return rows(x) != rows(y) ? rows(x) > rows(y) : x < y; });
+    int longest = 1;
+    for (int i = 0; i < plan.n; ++i) {
+        const int s = plan.seq[i];
+        plan.n_qt[i] = (tab.tok0[s + 1] - tab.tok0[s] + bt - 1) / bt;
+        longest = std::max(longest, (rows(s) + kBN - 1) / kBN);
+    }
+    long best = -1;
+    plan.chunk = longest;
+    for (int chunk = longest; chunk >= 1; chunk = chunk > 16 ? chunk * 7 / 8 : chunk - 1) {
+        long work = 0, parts = 0;
+        for (int i = 0; i < plan.n; ++i) {
+            const int s = plan.seq[i];
+            const long tiles = (rows(s) + kBN - 1) / kBN, ns = (tiles + chunk - 1) / chunk;
+            // causal tiles see from pos + bt rows on to all of them
+            const long mean = tree ? tiles : (tiles + (tab.pos[s] + bt + kBN - 1) / kBN + 1) / 2;
+            work += plan.n_qt[i] * (mean + ns * kOverhead + (ns > 1 ? ns : 0));
+            if (ns > 1) parts += plan.n_qt[i] * ns;
+        }
+        if (parts * c->n_kv > c->q8_tc_parts) break;
+        const long cost = work * c->n_kv / c->num_sms + chunk + kOverhead + (parts ? 2 : 0);
+        if (best < 0 || cost < best) {
+            best = cost;
+            plan.chunk = chunk;
+        }
+    }
+    int items = 0, tiles = 0, parts = 0;
+    for (int i = 0; i < plan.n; ++i) {
+        const int s = plan.seq[i];
+        const int ns = ((rows(s) + kBN - 1) / kBN + plan.chunk - 1) / plan.chunk;
+        plan.nsplit[i] = ns;
+        plan.item0[i] = items;
+        plan.tile0[i] = tiles;
+        plan.part0[i] = parts;
+        items += plan.n_qt[i] * ns;
+        tiles += plan.n_qt[i];
+        if (ns > 1) parts += plan.n_qt[i] * ns;
+    }
+    plan.item0[plan.n] = items;
+    plan.tile0[plan.n] = tiles;
+    plan.n_parts = parts;
+}
+
+}  // namespace
+
+int q8_tc_attend(leap_ctx *c, int layer, const Q8Seqs &tab, const Q8Tree *tree, const float *q, float *out) {
+    Q8TcPlan plan;
+    plan_tc(c, tab, tree != nullptr, plan);
+    TcArgs a;
+    a.q = q;
+    a.out = out;
+    a.L = q8_layer(c, layer);
+    a.rope_cos = c->rope_cos;
+    a.rope_sin = c->rope_sin;
+    a.part_o = c->q8_tc_part_o;
+    a.part_ml = c->q8_tc_part_ml;
+    a.err = c->d_err;
+    a.scale_log2 = kLog2e / sqrtf(float(c->hd));
+    switch (c->hd * 100 + c->group) {
+        case 12801: return launch_tc_g<128, 1>(c, a, tab, plan, tree);
+        case 12802: return launch_tc_g<128, 2>(c, a, tab, plan, tree);
+        case 12804: return launch_tc_g<128, 4>(c, a, tab, plan, tree);
+        case 12808: return launch_tc_g<128, 8>(c, a, tab, plan, tree);
+        case 6401: return launch_tc_g<64, 1>(c, a, tab, plan, tree);
+        case 6402: return launch_tc_g<64, 2>(c, a, tab, plan, tree);
+        case 6404: return launch_tc_g<64, 4>(c, a, tab, plan, tree);
+        case 6408: return launch_tc_g<64, 8>(c, a, tab, plan, tree);
+        default:
+            set_error("unsupported head_dim %d / kv_mul %d", c->hd, c->group);
+            return LEAP_ERR_INVALID;
+    }
+}
+
+}  // namespace leap

@@ -37,6 +37,8 @@ struct leap_ctx {
     float *q8_part_o = nullptr, *q8_part_ml = nullptr;  // [q8_parts][8][hd], [q8_parts][8][2]
     unsigned *q8_counters = nullptr;                    // [kMaxSeqPerLaunch][n_kv]
     int q8_parts = 0;
+    float *q8_tc_part_o = nullptr, *q8_tc_part_ml = nullptr;  // of 128 rows
+    int q8_tc_parts = 0;
 
     // RoPE table [max_seq][hd/2]
     float *rope_cos = nullptr, *rope_sin = nullptr;
@@ -171,6 +173,16 @@ struct Q8Splits {
     int chunk;
     int split0[kMaxSeqPerLaunch + 1];
 };
+// Blocks of the tensor-core kernel: entry i is sequence seq[i] (those without
+// tokens left out, longest first), n_qt[i] query tiles of 128 rows, each over
+// nsplit[i] splits of `chunk` key tiles.
+struct Q8TcPlan {
+    int n, chunk, n_parts;
+    int seq[kMaxSeqPerLaunch], n_qt[kMaxSeqPerLaunch], nsplit[kMaxSeqPerLaunch];
+    int part0[kMaxSeqPerLaunch];      // partials of split tiles, before this one
+    int item0[kMaxSeqPerLaunch + 1];  // (tile, split) pairs before it
+    int tile0[kMaxSeqPerLaunch + 1];  // tiles before it
+};
 constexpr int kQ8Rows = 8;  // query rows (tokens x heads of a group) of the rows kernel
 
 // One layer of the cache as kernels see it.
@@ -197,6 +209,9 @@ int kv_keep(leap_ctx *c, const Q8Seqs &tab, const Q8Tree &nodes);
 int q8_rows_parts(const leap_ctx *c);
 int q8_rows_attend(leap_ctx *c, int layer, const Q8Seqs &tab, const Q8Tree *tree, const float *q,
                    const float *k, const float *v, float *out);
+// The run's rows are stored already.
+int q8_tc_attend(leap_ctx *c, int layer, const Q8Seqs &tab, const Q8Tree *tree, const float *q,
+                 float *out);
 // Append and attend: causal, or a tree of each sequence's tokens.
 int q8_attend(leap_ctx *c, int layer, const Q8Seqs &tab, const Q8Tree *tree, const float *q,
               const float *k, const float *v, float *out);

@@ -212,7 +212,7 @@ Q8Layer q8_layer(const leap_ctx *c, int layer) {
 }
 
 int q8_create(leap_ctx *c) {
-    c->head_rows = c->max_seq_pad;
+    c->head_rows = (c->max_seq + 127) / 128 * 128;  // whole tiles can be read
     c->layer_rows = c->n_kv * c->head_rows;
     c->slot_rows = c->n_layers * c->layer_rows;
     const size_t rows = c->max_batch * c->slot_rows;
@@ -228,9 +228,13 @@ int q8_create(leap_ctx *c) {
     if (e == cudaSuccess) e = cudaMalloc(&c->q8_part_o, part * c->hd);
     if (e == cudaSuccess) e = cudaMalloc(&c->q8_part_ml, part * 2);
     if (e == cudaSuccess) e = cudaMalloc(&c->q8_counters, cnt);
+    c->q8_tc_parts = 4 * c->num_sms;
+    const size_t tc_part = size_t(c->q8_tc_parts) * 128 * sizeof(float);
+    if (e == cudaSuccess) e = cudaMalloc(&c->q8_tc_part_o, tc_part * c->hd);
+    if (e == cudaSuccess) e = cudaMalloc(&c->q8_tc_part_ml, tc_part * 2);
     if (e == cudaSuccess) e = cudaMemset(c->q8_counters, 0, cnt);
     if (e != cudaSuccess) return cuda_status(e, "cudaMalloc(8-bit cache)");
-    c->device_bytes += 2 * rows * (c->hd + sizeof(float)) + stage + part * (c->hd + 2) + cnt;
+    c->device_bytes += 2 * rows * (c->hd + sizeof(float)) + stage + (part + tc_part) * (c->hd + 2) + cnt;
     return q8_clear(c);
 }
 
@@ -243,6 +247,8 @@ void q8_free(leap_ctx *c) {
     cudaFree(c->q8_part_o);
     cudaFree(c->q8_part_ml);
     cudaFree(c->q8_counters);
+    cudaFree(c->q8_tc_part_o);
+    cudaFree(c->q8_tc_part_ml);
 }
 
 int q8_clear(leap_ctx *c) {

@@ -164,6 +164,21 @@ __device__ __forceinline__ void st16u(uint32_t taddr, const uint32_t (&v)[16]) {
         : "memory");
 }
 
+// The same reading 16 columns.
+__device__ __forceinline__ void ld16(uint32_t taddr, float (&v)[16]) {
+    uint32_t r[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
+          "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+
 // 32-bit instruction descriptor for kind::f16 with BF16 A and B (format 1),
 // F32 accumulate, both K-major, dense (the layout of idesc_tf32).
 __host__ __device__ constexpr uint32_t idesc_bf16(int M, int N) {
@@ -181,6 +196,32 @@ __device__ __forceinline__ void mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
         :
         : "r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// The same instruction descriptor with FP16 A and B (format 0); b_mn: B is
+// N-major (bit 16) instead of K-major.
+__host__ __device__ constexpr uint32_t idesc_f16(int M, int N, bool b_mn) {
+    return (1u << 4) | (b_mn ? 1u << 16 : 0u) | (uint32_t(N >> 3) << 17) | (uint32_t(M >> 4) << 24);
+}
+
+// Descriptor of an N-major operand with the 128-byte swizzle: rows (k) of 64
+// 16-bit values, the chunks of a row `chunk_bytes` apart (leading offset),
+// 8-row groups 1024 bytes apart (stride offset).
+__device__ __forceinline__ uint64_t sw128_nmajor_desc(uint32_t smem_byte_addr, uint32_t chunk_bytes) {
+    return uint64_t((smem_byte_addr >> 4) & 0x3FFFu) | uint64_t((chunk_bytes >> 4) & 0x3FFFu) << 16 |
+           uint64_t((1024u >> 4) & 0x3FFFu) << 32 | uint64_t(1u) << 46 | uint64_t(2u) << 61;
+}
+
+// D[tmem] (+)= A[smem desc] . B[smem desc], kind::f16 (K = 16 per product).
+__device__ __forceinline__ void mma_f16_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                           uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        :
+        : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
 
