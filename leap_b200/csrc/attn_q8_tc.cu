@@ -33,6 +33,7 @@
 // joined by a second kernel.
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "q8.cuh"
 #include "tc.cuh"
@@ -109,6 +110,13 @@ __device__ __forceinline__ uint4 expand(uint32_t a, uint32_t b) {
         return *reinterpret_cast<const uint32_t *>(&h);
     };
     return make_uint4(two(a, 0x5140), two(a, 0x5342), two(b, 0x5140), two(b, 0x5342));
+}
+
+// The largest of three (NaN counts as absent), one instruction.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
 
 template <int N>
@@ -216,7 +224,8 @@ q8_tc_kernel(const TcArgs a, const __grid_constant__ Q8Seqs tab, const __grid_co
                     // largest value to [2^14, 2^15); an infinite or NaN query gives NaN
                     const int ex = min(max(int(__reduce_max_sync(0xffffffffu, __float_as_uint(top)) >> 23), 15), 254);
                     const float up = __uint_as_float(uint32_t(268 - ex) << 23);
-                    const uint32_t off = tc::sw128_offset_b16(r, E * lane, kBM);
+                    // dims 64-127 in the converters' order: neighbouring granules swapped
+                    const uint32_t off = tc::sw128_offset_b16(r, E * lane, kBM) ^ (E * lane >= 64 ? 16u : 0u);
 #pragma unroll
                     for (int e = 0; e < E; e += 2) {
                         const float y0 = x[u][e] * up, y1 = x[u][e + 1] * up;
@@ -280,67 +289,78 @@ q8_tc_kernel(const TcArgs a, const __grid_constant__ Q8Seqs tab, const __grid_co
             const float4 *ks = reinterpret_cast<const float4 *>(s_ks[slot]);
             const float4 *vs = reinterpret_cast<const float4 *>(s_vs[slot]);
             const bool full = __all_sync(0xffffffffu, (TREE ? pos : lim) >= k0 + kBN);
-            // the largest score (in units of 1/fac)
-            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-                float s[32];
-                tc::ld32(scol + 32 * c, s);
-                tc::wait_ld();
-                const uint32_t vis = full ? ~0u : seen(k0 + 32 * c);
+            // Two passes over S in steps of 16 keys, the next step's read in
+            // flight: the largest score (in units of 1/fac), then the weights.
+            float alpha;
+            float s[2][16];
+            auto softmax = [&](auto all_seen) {
+                constexpr bool FULL = decltype(all_seen)::value;
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                tc::ld16_async(scol, s[0]);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float4 f = ks[8 * c + i];
-                    const float2 x = __fmul2_rn(make_float2(s[4 * i], s[4 * i + 1]), make_float2(f.x, f.y));
-                    const float2 y = __fmul2_rn(make_float2(s[4 * i + 2], s[4 * i + 3]), make_float2(f.z, f.w));
-                    if (full) {
-                        mx[0] = fmaxf(mx[0], x.x);
-                        mx[1] = fmaxf(mx[1], x.y);
-                        mx[2] = fmaxf(mx[2], y.x);
-                        mx[3] = fmaxf(mx[3], y.y);
-                    } else {
-                        if (vis >> (4 * i) & 1) mx[0] = fmaxf(mx[0], x.x);
-                        if (vis >> (4 * i + 1) & 1) mx[1] = fmaxf(mx[1], x.y);
-                        if (vis >> (4 * i + 2) & 1) mx[2] = fmaxf(mx[2], y.x);
-                        if (vis >> (4 * i + 3) & 1) mx[3] = fmaxf(mx[3], y.y);
+                for (int c = 0; c < kBN / 16; ++c) {
+                    float(&x)[16] = s[c & 1];
+                    tc::wait_ld16(x);
+                    tc::ld16_async(scol + (c + 1 < kBN / 16 ? 16 * (c + 1) : 0), s[(c + 1) & 1]);
+                    const uint32_t vis = FULL ? ~0u : seen(k0 + 16 * c);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float4 f = ks[4 * c + i];
+                        float2 y = __fmul2_rn(make_float2(x[4 * i], x[4 * i + 1]), make_float2(f.x, f.y));
+                        float2 z = __fmul2_rn(make_float2(x[4 * i + 2], x[4 * i + 3]), make_float2(f.z, f.w));
+                        if (!FULL) {
+                            if (!(vis >> (4 * i) & 1)) y.x = -INFINITY;
+                            if (!(vis >> (4 * i + 1) & 1)) y.y = -INFINITY;
+                            if (!(vis >> (4 * i + 2) & 1)) z.x = -INFINITY;
+                            if (!(vis >> (4 * i + 3) & 1)) z.y = -INFINITY;
+                        }
+                        mx[i & 1] = max3(mx[i & 1], y.x, y.y);
+                        mx[2 + (i & 1)] = max3(mx[2 + (i & 1)], z.x, z.y);
                     }
                 }
-            }
-            const float mn = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * fac);
-            const float ref = mn == -INFINITY ? 0.f : mn;  // nothing seen so far
-            const float alpha = fast_exp2(m - ref);
-            m = mn;
-            const float2 fac2 = make_float2(fac, fac), nref2 = make_float2(-ref, -ref);
-            float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll 1
-            for (int c = 0; c < kBN / 16; ++c) {  // 16 keys: one step of the PV product
-                float s[16];
-                tc::ld16(scol + 16 * c, s);
-                tc::wait_ld();
-                const uint32_t vis = full ? ~0u : seen(k0 + 16 * c);
-                uint32_t hl[16];  // 8 words hi, 8 words lo: over the scores they come from
+                const float mn = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * fac);
+                const float ref = mn == -INFINITY ? 0.f : mn;  // nothing seen so far
+                alpha = fast_exp2(m - ref);
+                m = mn;
+                const float2 fac2 = make_float2(fac, fac), nref2 = make_float2(-ref, -ref);
+                float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float2 f = reinterpret_cast<const float2 *>(ks)[8 * c + i];
-                    const float2 g = reinterpret_cast<const float2 *>(vs)[8 * c + i];
-                    const float2 e = __ffma2_rn(__fmul2_rn(make_float2(s[2 * i], s[2 * i + 1]), f), fac2, nref2);
-                    float2 p = make_float2(fast_exp2(e.x), fast_exp2(e.y));
-                    float2 w = __fmul2_rn(p, g);
-                    if (!full) {  // what is not seen takes no part, whatever its scales
-                        if (!(vis >> (2 * i) & 1)) p.x = w.x = 0.f;
-                        if (!(vis >> (2 * i + 1) & 1)) p.y = w.y = 0.f;
+                for (int c = 0; c < kBN / 16; ++c) {  // 16 keys: one step of the PV product
+                    float(&x)[16] = s[c & 1];
+                    tc::wait_ld16(x);
+                    if (c + 1 < kBN / 16) tc::ld16_async(scol + 16 * (c + 1), s[(c + 1) & 1]);
+                    const uint32_t vis = FULL ? ~0u : seen(k0 + 16 * c);
+                    uint32_t hl[16];  // 8 words hi, 8 words lo: over the scores they come from
+#pragma unroll
+                    for (int i = 0; i < 8; i += 2) {
+                        const float4 f = ks[4 * c + i / 2], g = vs[4 * c + i / 2];
+                        const float2 f2[2] = {make_float2(f.x, f.y), make_float2(f.z, f.w)};
+                        const float2 g2[2] = {make_float2(g.x, g.y), make_float2(g.z, g.w)};
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            const int k = 2 * (i + u);
+                            const float2 e = __ffma2_rn(__fmul2_rn(make_float2(x[k], x[k + 1]), f2[u]), fac2, nref2);
+                            float2 p = make_float2(fast_exp2(e.x), fast_exp2(e.y));
+                            float2 w = __fmul2_rn(p, g2[u]);
+                            if (!FULL) {  // what is not seen takes no part, whatever its scales
+                                if (!(vis >> k & 1)) p.x = w.x = 0.f;
+                                if (!(vis >> (k + 1) & 1)) p.y = w.y = 0.f;
+                            }
+                            sum[u] = __fadd2_rn(sum[u], p);
+                            const __half2 hi = __floats2half2_rn(w.x, w.y);
+                            const float2 back = __half22float2(hi);
+                            const float2 r = __fadd2_rn(w, make_float2(-back.x, -back.y));
+                            const __half2 lo = __floats2half2_rn(r.x, r.y);
+                            hl[i + u] = *reinterpret_cast<const uint32_t *>(&hi);
+                            hl[8 + i + u] = *reinterpret_cast<const uint32_t *>(&lo);
+                        }
                     }
-                    sum[i & 1] = __fadd2_rn(sum[i & 1], p);
-                    const __half2 hi = __floats2half2_rn(w.x, w.y);
-                    const float2 back = __half22float2(hi);
-                    const float2 r = __fadd2_rn(w, make_float2(-back.x, -back.y));
-                    const __half2 lo = __floats2half2_rn(r.x, r.y);
-                    hl[i] = *reinterpret_cast<const uint32_t *>(&hi);
-                    hl[8 + i] = *reinterpret_cast<const uint32_t *>(&lo);
+                    tc::st16u(scol + 16 * c, hl);
                 }
-                tc::st16u(scol + 16 * c, hl);
-            }
-            l = l * alpha + ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
+                l = l * alpha + ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
+            };
+            if (full) softmax(std::true_type());
+            else softmax(std::false_type());
             const float vdown = s_vdown[slot];
             tc::wait_st();
             tc::fence_before_sync();
@@ -349,20 +369,29 @@ q8_tc_kernel(const TcArgs a, const __grid_constant__ Q8Seqs tab, const __grid_co
             ok = __all_sync(0xffffffffu, mbar_wait(&bars.o_full[b], par(j)));
             if (!ok) break;
             tc::fence_after_sync();
+            // o = o * alpha + O(j) * vdown; most tiles move no row's maximum
             const float2 al2 = make_float2(alpha, alpha), vd2 = make_float2(vdown, vdown);
+            const bool still = __all_sync(0xffffffffu, alpha == 1.f);
+            const uint32_t ocol = tmem + lane_off + C::kColO(b);
+            auto add = [&](auto no_move) {
+                tc::ld16_async(ocol, s[0]);
 #pragma unroll
-            for (int c = 0; c < HD / 32; ++c) {
-                float x[32];
-                tc::ld32(tmem + lane_off + C::kColO(b) + 32 * c, x);
-                tc::wait_ld();
+                for (int c = 0; c < HD / 16; ++c) {
+                    float(&x)[16] = s[c & 1];
+                    tc::wait_ld16(x);
+                    if (c + 1 < HD / 16) tc::ld16_async(ocol + 16 * (c + 1), s[(c + 1) & 1]);
 #pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                    const float2 z = __ffma2_rn(make_float2(x[i], x[i + 1]), vd2,
-                                                __fmul2_rn(make_float2(o[32 * c + i], o[32 * c + i + 1]), al2));
-                    o[32 * c + i] = z.x;
-                    o[32 * c + i + 1] = z.y;
+                    for (int i = 0; i < 16; i += 2) {
+                        float2 y = make_float2(o[16 * c + i], o[16 * c + i + 1]);
+                        if (!decltype(no_move)::value) y = __fmul2_rn(y, al2);
+                        y = __ffma2_rn(make_float2(x[i], x[i + 1]), vd2, y);
+                        o[16 * c + i] = y.x;
+                        o[16 * c + i + 1] = y.y;
+                    }
                 }
-            }
+            };
+            if (still) add(std::true_type());
+            else add(std::false_type());
             tc::fence_before_sync();  // O(j) read before PV(j+2), which p_full(j+2) allows
         }
         if (!ok && lane == 0) atomicExch(&s_fail, 1);
@@ -390,19 +419,20 @@ q8_tc_kernel(const TcArgs a, const __grid_constant__ Q8Seqs tab, const __grid_co
 #pragma unroll
                 for (int i = 0; i < HD / 4; ++i) {
                     const float4 x = s_o[i * kBM + row];
+                    const int d4 = i < 16 ? i : i ^ 2;  // columns 64-127: 8-dim granules swapped
                     float4 v;
                     v.x = (o[4 * i] * e0 + x.x * e1) * inv;
                     v.y = (o[4 * i + 1] * e0 + x.y * e1) * inv;
                     v.z = (o[4 * i + 2] * e0 + x.z * e1) * inv;
                     v.w = (o[4 * i + 3] * e0 + x.w * e1) * inv;
-                    if (tok < t_end) *reinterpret_cast<float4 *>(dst + 4 * i) = v;
+                    if (tok < t_end) *reinterpret_cast<float4 *>(dst + 4 * d4) = v;
                 }
             } else if (tok < t_end) {
                 float4 *po = reinterpret_cast<float4 *>(a.part_o) + size_t(it.part) * (HD / 4) * kBM + row;
 #pragma unroll
                 for (int i = 0; i < HD / 4; ++i) {
                     const float4 x = s_o[i * kBM + row];
-                    po[i * kBM] = make_float4(o[4 * i] * e0 + x.x * e1, o[4 * i + 1] * e0 + x.y * e1,
+                    po[(i < 16 ? i : i ^ 2) * kBM] = make_float4(o[4 * i] * e0 + x.x * e1, o[4 * i + 1] * e0 + x.y * e1,
                                               o[4 * i + 2] * e0 + x.z * e1, o[4 * i + 3] * e0 + x.w * e1);
                 }
                 reinterpret_cast<float2 *>(a.part_ml)[size_t(it.part) * kBM + row] = make_float2(mm, sum);
@@ -429,8 +459,9 @@ q8_tc_kernel(const TcArgs a, const __grid_constant__ Q8Seqs tab, const __grid_co
         };
         // Chunk ct + 128 i (16 bytes each) of a tile: its line is (ct >> 3) + 16 i,
         // so its dims and its place in an 8-row swizzle group are the same for
-        // every i.  Chunks 4-7 store their upper half first: eight neighbouring
-        // threads then meet eight different bank groups.
+        // every i.  Chunks 4-7 have their two 8-dim granules swapped, so that
+        // eight neighbouring threads meet eight different bank groups; Q's dims
+        // 64-127 and O's columns 64-127 are in that order too.
         int row, ch;
         if (HD == 128) {
             row = ct >> 3;
@@ -449,8 +480,8 @@ q8_tc_kernel(const TcArgs a, const __grid_constant__ Q8Seqs tab, const __grid_co
 #pragma unroll
             for (int i = 0; i < N2; ++i) {
                 const uint4 x = w[half][i];
-                *reinterpret_cast<uint4 *>(d0 + i * kStep) = expand(upper ? x.z : x.x, upper ? x.w : x.y);
-                *reinterpret_cast<uint4 *>(d1 + i * kStep) = expand(upper ? x.x : x.z, upper ? x.y : x.w);
+                *reinterpret_cast<uint4 *>(d0 + i * kStep) = expand(x.x, x.y);
+                *reinterpret_cast<uint4 *>(d1 + i * kStep) = expand(x.z, x.w);
             }
         };
         bool ok = true;
