@@ -18,16 +18,14 @@
 //
 // Roles (16 warps; registers moved to where O lives by setmaxnreg, 200 + 200 +
 // 72 + 40 = 4 x 128):
-//   warps 0-3, 4-7   two softmax groups; group b takes tiles b, b+2, ...: S(j)
-//                    from TMEM, p, hi/lo back over S in place, then O(j) into
-//                    its registers.  Each keeps its own maximum, sum and output;
-//                    the two are joined at the end.  While one waits for its
-//                    PV product the other works.
+//   warps 0-7        softmax, two threads a row (64 keys and half of O's columns
+//                    each): S(j) from TMEM, p, hi/lo back over S in place; then
+//                    O(j-1), whose product ran meanwhile, into registers.
 //   warps 8-11       codes -> FP16 operand tiles (128-byte swizzle; V is used
 //                    N-major, so nothing is transposed), a tile ahead in
 //                    registers, and the tile's scales.
-//   warp 12          issues S(j) = Q K^T and O(j) = P V, whichever is ready.
-// TMEM: S/P and O of either group (2 x (128 + HD) columns).  Shared memory:
+//   warp 12          issues the products: S(j+1) = Q K^T, then O(j) = P V.
+// TMEM: two buffers each of S/P and O (2 x (128 + HD) columns).  Shared memory:
 // Q hi/lo, two buffers each of K and V.
 // Long ranges are split over blocks when a launch has few tiles; partials are
 // joined by a second kernel.
@@ -75,7 +73,7 @@ struct TcBars {
     uint64_t k_full[2], v_full[2];  // operand tile in place (4 converter warps)
     uint64_t sc_full[kSlots];       // scales of a tile in place (4 converter warps)
     uint64_t s_full[2];  // S(j) done: K buffer free (commit)
-    uint64_t p_full[2];  // P(j) in TMEM (4 softmax warps)
+    uint64_t p_full[2];  // P(j) in TMEM (8 softmax warps)
     uint64_t o_full[2];  // O(j) done: V buffer and S/P columns free (commit)
 };
 
@@ -124,6 +122,20 @@ __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.al
 template <int N>
 __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
+// Barrier of the 256 softmax threads (named barrier 1): true if `ok` everywhere.
+__device__ __forceinline__ bool group_and(bool ok) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %1, 0;\n\t"
+        "barrier.cta.red.and.pred q, 1, 256, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r)
+        : "r"(uint32_t(ok))
+        : "memory");
+    return r != 0;
+}
+
 template <int HD, int G, bool TREE>
 __global__ void __launch_bounds__(kThreads, 1)
 q8_tc_kernel(const TcArgs a, const __grid_constant__ Q8Seqs tab, const __grid_constant__ Q8TcPlan plan,
@@ -133,7 +145,7 @@ q8_tc_kernel(const TcArgs a, const __grid_constant__ Q8Seqs tab, const __grid_co
     extern __shared__ unsigned char smem_raw[];
     __shared__ TcBars bars;
     __shared__ __align__(16) float s_ks[kSlots][kBN], s_vs[kSlots][kBN];
-    __shared__ float s_vdown[kSlots], s_fac[kBM], s_m[kBM], s_l[kBM];
+    __shared__ float s_vdown[kSlots], s_fac[kBM], s_mx[2][2][kBM], s_l[2][kBM];
     __shared__ int8_t s_parent[TREE ? kMaxTreeNodes : 1];
     __shared__ uint32_t s_anc[TREE ? 4 : 1][kBM];  // TREE: what each row sees of the run
     __shared__ uint32_t tmem_sh;
@@ -159,7 +171,7 @@ q8_tc_kernel(const TcArgs a, const __grid_constant__ Q8Seqs tab, const __grid_co
             mbar_init(&bars.k_full[b], 4);
             mbar_init(&bars.v_full[b], 4);
             mbar_init(&bars.s_full[b], 1);
-            mbar_init(&bars.p_full[b], 4);
+            mbar_init(&bars.p_full[b], 8);
             mbar_init(&bars.o_full[b], 1);
         }
         for (int i = 0; i < kSlots; ++i) mbar_init(&bars.sc_full[i], 4);
@@ -180,7 +192,9 @@ q8_tc_kernel(const TcArgs a, const __grid_constant__ Q8Seqs tab, const __grid_co
     if (warp < 8) {
         // ================= softmax groups =====================================
         regs_up<kRegsSoftmax>();
-        const int b = warp >> 2;             // group
+        // Two threads a row: half 0 has keys 0-63 of a tile and the lower half of
+        // O's columns, half 1 the rest.
+        const int half = warp >> 2;
         const int row = tid & 127;           // TMEM lane
         const uint32_t lane_off = uint32_t((warp & 3) * 32) << 16;
         // Q was written before the append kernel began, so it needs no wait
@@ -248,7 +262,7 @@ q8_tc_kernel(const TcArgs a, const __grid_constant__ Q8Seqs tab, const __grid_co
         // those of the run whose bit is set (itself and its ancestors).
         const int tok = t0 + row / G;
         const int lim = pos + min(tok, t_end - 1) + 1;
-        if (TREE && b == 0) {
+        if (TREE && half == 0) {
             uint32_t anc[4] = {0u, 0u, 0u, 0u};
             for (int p = min(tok, t_end - 1); p >= 0; p = s_parent[p]) {
 #pragma unroll
@@ -258,7 +272,7 @@ q8_tc_kernel(const TcArgs a, const __grid_constant__ Q8Seqs tab, const __grid_co
 #pragma unroll
             for (int w = 0; w < 4; ++w) s_anc[w][row] = anc[w];
         }
-        if (TREE) asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (TREE) ok = group_and(ok);
         // bit i: whether key k0 + i is seen
         auto seen = [&](int k0) -> uint32_t {
             if (!TREE) {
@@ -272,170 +286,178 @@ q8_tc_kernel(const TcArgs a, const __grid_constant__ Q8Seqs tab, const __grid_co
         };
 
         const float fac = s_fac[row];
+        constexpr int OC = HD / 2;           // O columns of a thread
         float m = -INFINITY, l = 0.f;
-        float o[HD];
+        float o[OC];
 #pragma unroll
-        for (int i = 0; i < HD; ++i) o[i] = 0.f;
+        for (int i = 0; i < OC; ++i) o[i] = 0.f;
 
-        for (int j = b; j < n_kt && ok; j += 2) {
-            ok = mbar_wait(&bars.sc_full[j & (kSlots - 1)], uint32_t(j / kSlots) & 1u) &&
+        // o = o * alpha + O(j) * vdown, in FP32; most tiles move no row's maximum
+        auto absorb = [&](int j, float alpha, float vdown) -> bool {
+            const bool there = __all_sync(0xffffffffu, mbar_wait(&bars.o_full[j & 1], par(j)));
+            if (!there) return false;
+            tc::fence_after_sync();
+            const uint32_t ocol = tmem + lane_off + C::kColO(j & 1) + half * OC;
+            const float2 al2 = make_float2(alpha, alpha), vd2 = make_float2(vdown, vdown);
+            auto add = [&](auto still) {
+                float x[2][16];
+                tc::ld16_async(ocol, x[0]);
+#pragma unroll
+                for (int c = 0; c < OC / 16; ++c) {
+                    float(&y)[16] = x[c & 1];
+                    tc::wait_ld16(y);
+                    if (c + 1 < OC / 16) tc::ld16_async(ocol + 16 * (c + 1), x[(c + 1) & 1]);
+#pragma unroll
+                    for (int i = 0; i < 16; i += 2) {
+                        float2 z = make_float2(o[16 * c + i], o[16 * c + i + 1]);
+                        if (!decltype(still)::value) z = __fmul2_rn(z, al2);
+                        z = __ffma2_rn(make_float2(y[i], y[i + 1]), vd2, z);
+                        o[16 * c + i] = z.x;
+                        o[16 * c + i + 1] = z.y;
+                    }
+                }
+            };
+            if (__all_sync(0xffffffffu, alpha == 1.f)) add(std::true_type());
+            else add(std::false_type());
+            return true;
+        };
+
+        float alpha = 1.f, vdown = 0.f;      // of the tile whose O is still to come
+        for (int j = 0; j < n_kt; ++j) {
+            const int b = j & 1, slot = j & (kSlots - 1);
+            ok = ok && mbar_wait(&bars.sc_full[slot], uint32_t(j / kSlots) & 1u) &&
                  mbar_wait(&bars.s_full[b], par(j));
             ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
             tc::fence_after_sync();
-            const int slot = j & (kSlots - 1);
-            const int k0 = (j0 + j) * kBN;
-            const uint32_t scol = tmem + lane_off + C::kColS(b);
-            const float4 *ks = reinterpret_cast<const float4 *>(s_ks[slot]);
-            const float4 *vs = reinterpret_cast<const float4 *>(s_vs[slot]);
-            const bool full = __all_sync(0xffffffffu, (TREE ? pos : lim) >= k0 + kBN);
-            // Two passes over S in steps of 16 keys, the next step's read in
-            // flight: the largest score (in units of 1/fac), then the weights.
-            float alpha;
-            float s[2][16];
-            auto softmax = [&](auto all_seen) {
-                constexpr bool FULL = decltype(all_seen)::value;
-                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                tc::ld16_async(scol, s[0]);
+            const int k0 = (j0 + j) * kBN + 64 * half;
+            const uint32_t scol = tmem + lane_off + C::kColS(b) + 64 * half;
+            const float4 *ks = reinterpret_cast<const float4 *>(s_ks[slot]) + 16 * half;
+            const float4 *vs = reinterpret_cast<const float4 *>(s_vs[slot]) + 16 * half;
+            const bool full = __all_sync(0xffffffffu, (TREE ? pos : lim) >= k0 + 64);
+            const uint2 vis = full ? make_uint2(~0u, ~0u) : make_uint2(seen(k0), seen(k0 + 32));
+            // scores in units of 1/fac, and the largest of the thread's half
+            float s[4][16];
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int c = 0; c < kBN / 16; ++c) {
-                    float(&x)[16] = s[c & 1];
-                    tc::wait_ld16(x);
-                    tc::ld16_async(scol + (c + 1 < kBN / 16 ? 16 * (c + 1) : 0), s[(c + 1) & 1]);
-                    const uint32_t vis = FULL ? ~0u : seen(k0 + 16 * c);
+            for (int c = 0; c < 4; ++c) tc::ld16_async(scol + 16 * c, s[c]);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float4 f = ks[4 * c + i];
-                        float2 y = __fmul2_rn(make_float2(x[4 * i], x[4 * i + 1]), make_float2(f.x, f.y));
-                        float2 z = __fmul2_rn(make_float2(x[4 * i + 2], x[4 * i + 3]), make_float2(f.z, f.w));
-                        if (!FULL) {
-                            if (!(vis >> (4 * i) & 1)) y.x = -INFINITY;
-                            if (!(vis >> (4 * i + 1) & 1)) y.y = -INFINITY;
-                            if (!(vis >> (4 * i + 2) & 1)) z.x = -INFINITY;
-                            if (!(vis >> (4 * i + 3) & 1)) z.y = -INFINITY;
-                        }
-                        mx[i & 1] = max3(mx[i & 1], y.x, y.y);
-                        mx[2 + (i & 1)] = max3(mx[2 + (i & 1)], z.x, z.y);
-                    }
+            for (int c = 0; c < 4; ++c) {
+                tc::wait_ld16(s[c]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float4 f = ks[4 * c + i];
+                    const float2 y = __fmul2_rn(make_float2(s[c][4 * i], s[c][4 * i + 1]), make_float2(f.x, f.y));
+                    const float2 z = __fmul2_rn(make_float2(s[c][4 * i + 2], s[c][4 * i + 3]), make_float2(f.z, f.w));
+                    s[c][4 * i] = y.x;
+                    s[c][4 * i + 1] = y.y;
+                    s[c][4 * i + 2] = z.x;
+                    s[c][4 * i + 3] = z.y;
                 }
-                const float mn = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * fac);
-                const float ref = mn == -INFINITY ? 0.f : mn;  // nothing seen so far
-                alpha = fast_exp2(m - ref);
-                m = mn;
-                const float2 fac2 = make_float2(fac, fac), nref2 = make_float2(-ref, -ref);
-                float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+            }
+            if (!full) {
 #pragma unroll
-                for (int c = 0; c < kBN / 16; ++c) {  // 16 keys: one step of the PV product
-                    float(&x)[16] = s[c & 1];
-                    tc::wait_ld16(x);
-                    if (c + 1 < kBN / 16) tc::ld16_async(scol + 16 * (c + 1), s[(c + 1) & 1]);
-                    const uint32_t vis = FULL ? ~0u : seen(k0 + 16 * c);
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (!((c < 2 ? vis.x : vis.y) >> ((16 * c + i) & 31) & 1)) s[c][i] = -INFINITY;
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], s[c][i], s[c][i + 1]);
+            const float mine = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
+            // The row's other half; the barrier also carries a wait that gave up,
+            // so that all leave together.  (s_mx alternates: a slow thread may
+            // still read the tile before.)
+            s_mx[b][half][row] = mine;
+            ok = group_and(ok);
+            if (!ok) break;
+            const float mn = fmaxf(m, fmaxf(mine, s_mx[b][half ^ 1][row]) * fac);
+            const float ref = mn == -INFINITY ? 0.f : mn;  // nothing seen so far
+            const float al = fast_exp2(m - ref);
+            m = mn;
+            const float2 fac2 = make_float2(fac, fac), nref2 = make_float2(-ref, -ref);
+            float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+            // s becomes p a step of 16 keys (one of the PV product) ahead of the
+            // split into halves, so that exponentials and the rest overlap.
+            auto weights = [&](auto all_seen) {
+                constexpr bool FULL = decltype(all_seen)::value;
+                uint32_t off[4] = {0u, 0u, 0u, 0u};  // !FULL: keys that are not seen
+                auto exps = [&](int c) {
+#pragma unroll
+                    for (int i = 0; i < 16; i += 2) {
+                        const float2 e = __ffma2_rn(make_float2(s[c][i], s[c][i + 1]), fac2, nref2);
+                        if (!FULL) {
+                            off[c] |= (s[c][i] == -INFINITY ? 1u << i : 0u) | (s[c][i + 1] == -INFINITY ? 2u << i : 0u);
+                        }
+                        s[c][i] = fast_exp2(e.x);
+                        s[c][i + 1] = fast_exp2(e.y);
+                    }
+                };
+                exps(0);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    if (c + 1 < 4) exps(c + 1);
                     uint32_t hl[16];  // 8 words hi, 8 words lo: over the scores they come from
 #pragma unroll
-                    for (int i = 0; i < 8; i += 2) {
-                        const float4 f = ks[4 * c + i / 2], g = vs[4 * c + i / 2];
-                        const float2 f2[2] = {make_float2(f.x, f.y), make_float2(f.z, f.w)};
-                        const float2 g2[2] = {make_float2(g.x, g.y), make_float2(g.z, g.w)};
-#pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            const int k = 2 * (i + u);
-                            const float2 e = __ffma2_rn(__fmul2_rn(make_float2(x[k], x[k + 1]), f2[u]), fac2, nref2);
-                            float2 p = make_float2(fast_exp2(e.x), fast_exp2(e.y));
-                            float2 w = __fmul2_rn(p, g2[u]);
-                            if (!FULL) {  // what is not seen takes no part, whatever its scales
-                                if (!(vis >> k & 1)) p.x = w.x = 0.f;
-                                if (!(vis >> (k + 1) & 1)) p.y = w.y = 0.f;
-                            }
-                            sum[u] = __fadd2_rn(sum[u], p);
-                            const __half2 hi = __floats2half2_rn(w.x, w.y);
-                            const float2 back = __half22float2(hi);
-                            const float2 r = __fadd2_rn(w, make_float2(-back.x, -back.y));
-                            const __half2 lo = __floats2half2_rn(r.x, r.y);
-                            hl[i + u] = *reinterpret_cast<const uint32_t *>(&hi);
-                            hl[8 + i + u] = *reinterpret_cast<const uint32_t *>(&lo);
+                    for (int i = 0; i < 8; ++i) {
+                        const float4 g = vs[4 * c + i / 2];
+                        const float2 p = make_float2(s[c][2 * i], s[c][2 * i + 1]);
+                        float2 w = __fmul2_rn(p, i & 1 ? make_float2(g.z, g.w) : make_float2(g.x, g.y));
+                        if (!FULL) {  // what is not seen (p = 0) takes no part, whatever its scale
+                            if (off[c] >> (2 * i) & 1) w.x = 0.f;
+                            if (off[c] >> (2 * i + 1) & 1) w.y = 0.f;
                         }
+                        sum[i & 1] = __fadd2_rn(sum[i & 1], p);
+                        const __half2 hi = __floats2half2_rn(w.x, w.y);
+                        const float2 back = __half22float2(hi);
+                        const float2 r = __fadd2_rn(w, make_float2(-back.x, -back.y));
+                        const __half2 lo = __floats2half2_rn(r.x, r.y);
+                        hl[i] = *reinterpret_cast<const uint32_t *>(&hi);
+                        hl[8 + i] = *reinterpret_cast<const uint32_t *>(&lo);
                     }
-                    tc::st16u(scol + 16 * c, hl);
+                    tc::st16u_free(scol + 16 * c, hl);
                 }
-                l = l * alpha + ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
             };
-            if (full) softmax(std::true_type());
-            else softmax(std::false_type());
-            const float vdown = s_vdown[slot];
+            if (full) weights(std::true_type());
+            else weights(std::false_type());
+            l = l * al + ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
+            const float vd = s_vdown[slot];
             tc::wait_st();
             tc::fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars.p_full[b]);
-            ok = __all_sync(0xffffffffu, mbar_wait(&bars.o_full[b], par(j)));
-            if (!ok) break;
-            tc::fence_after_sync();
-            // o = o * alpha + O(j) * vdown; most tiles move no row's maximum
-            const float2 al2 = make_float2(alpha, alpha), vd2 = make_float2(vdown, vdown);
-            const bool still = __all_sync(0xffffffffu, alpha == 1.f);
-            const uint32_t ocol = tmem + lane_off + C::kColO(b);
-            auto add = [&](auto no_move) {
-                tc::ld16_async(ocol, s[0]);
-#pragma unroll
-                for (int c = 0; c < HD / 16; ++c) {
-                    float(&x)[16] = s[c & 1];
-                    tc::wait_ld16(x);
-                    if (c + 1 < HD / 16) tc::ld16_async(ocol + 16 * (c + 1), s[(c + 1) & 1]);
-#pragma unroll
-                    for (int i = 0; i < 16; i += 2) {
-                        float2 y = make_float2(o[16 * c + i], o[16 * c + i + 1]);
-                        if (!decltype(no_move)::value) y = __fmul2_rn(y, al2);
-                        y = __ffma2_rn(make_float2(x[i], x[i + 1]), vd2, y);
-                        o[16 * c + i] = y.x;
-                        o[16 * c + i + 1] = y.y;
-                    }
-                }
-            };
-            if (still) add(std::true_type());
-            else add(std::false_type());
-            tc::fence_before_sync();  // O(j) read before PV(j+2), which p_full(j+2) allows
+            // O(j-1), whose product ran beside this softmax
+            if (j > 0) ok = absorb(j - 1, alpha, vdown);
+            tc::fence_before_sync();  // read before PV(j+1), which p_full(j+1) allows
+            alpha = al;
+            vdown = vd;
         }
+        if (ok && n_kt > 0) ok = absorb(n_kt - 1, alpha, vdown);
         if (!ok && lane == 0) atomicExch(&s_fail, 1);
-        // ---- join the two groups: group 1's state through shared memory ---------
-        // (both groups are past their last tile here, so no buffer is in use;
-        // named barrier 1: the 256 threads of both)
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        float4 *s_o = reinterpret_cast<float4 *>(base + C::kK);  // [HD/4][128]
-        if (b == 1) {
-            s_m[row] = m;
-            s_l[row] = l;
-#pragma unroll
-            for (int i = 0; i < HD / 4; ++i)
-                s_o[i * kBM + row] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-        }
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        if (b == 0 && !*reinterpret_cast<volatile int *>(&s_fail)) {
-            const float m1 = s_m[row], mm = fmaxf(m, m1);
-            const float e0 = m == -INFINITY ? 0.f : fast_exp2(m - mm);
-            const float e1 = m1 == -INFINITY ? 0.f : fast_exp2(m1 - mm);
-            const float sum = l * e0 + s_l[row] * e1;
+        s_l[half][row] = l;
+        ok = group_and(ok);
+        if (ok && tok < t_end) {
+            const float sum = s_l[0][row] + s_l[1][row];
+            float4 *dst;
+            size_t step;
+            float by = 1.f;
             if (it.part < 0) {
-                const float inv = 1.f / sum;
-                float *dst = a.out + (size_t(tok0 + tok) * a.L.n_kv * G + h * G + row % G) * HD;
+                dst = reinterpret_cast<float4 *>(a.out + (size_t(tok0 + tok) * a.L.n_kv * G + h * G + row % G) * HD);
+                step = 1;
+                by = 1.f / sum;
+            } else {
+                dst = reinterpret_cast<float4 *>(a.part_o) + size_t(it.part) * (HD / 4) * kBM + row;
+                step = kBM;
+                if (half == 0)
+                    reinterpret_cast<float2 *>(a.part_ml)[size_t(it.part) * kBM + row] = make_float2(m, sum);
+            }
+            dst += half * (OC / 4) * step;
 #pragma unroll
-                for (int i = 0; i < HD / 4; ++i) {
-                    const float4 x = s_o[i * kBM + row];
-                    const int d4 = i < 16 ? i : i ^ 2;  // columns 64-127: 8-dim granules swapped
-                    float4 v;
-                    v.x = (o[4 * i] * e0 + x.x * e1) * inv;
-                    v.y = (o[4 * i + 1] * e0 + x.y * e1) * inv;
-                    v.z = (o[4 * i + 2] * e0 + x.z * e1) * inv;
-                    v.w = (o[4 * i + 3] * e0 + x.w * e1) * inv;
-                    if (tok < t_end) *reinterpret_cast<float4 *>(dst + 4 * d4) = v;
-                }
-            } else if (tok < t_end) {
-                float4 *po = reinterpret_cast<float4 *>(a.part_o) + size_t(it.part) * (HD / 4) * kBM + row;
-#pragma unroll
-                for (int i = 0; i < HD / 4; ++i) {
-                    const float4 x = s_o[i * kBM + row];
-                    po[(i < 16 ? i : i ^ 2) * kBM] = make_float4(o[4 * i] * e0 + x.x * e1, o[4 * i + 1] * e0 + x.y * e1,
-                                              o[4 * i + 2] * e0 + x.z * e1, o[4 * i + 3] * e0 + x.w * e1);
-                }
-                reinterpret_cast<float2 *>(a.part_ml)[size_t(it.part) * kBM + row] = make_float2(mm, sum);
+            for (int i = 0; i < OC / 4; ++i) {
+                // columns 64-127 have neighbouring 8-dim granules swapped
+                const int d4 = HD == 128 && half ? i ^ 2 : i;
+                dst[d4 * step] = make_float4(o[4 * i] * by, o[4 * i + 1] * by, o[4 * i + 2] * by, o[4 * i + 3] * by);
             }
         }
     } else if (warp < 12) {
@@ -542,62 +564,55 @@ q8_tc_kernel(const TcArgs a, const __grid_constant__ Q8Seqs tab, const __grid_co
             const uint64_t dk = tc::sw128_kmajor_desc(sbase + C::kK);
             const uint64_t dv = tc::sw128_nmajor_desc(sbase + C::kV, C::kChunk);
             int s_issued = 0, pv_issued = 0;
-            bool ok = __all_sync(0xffffffffu, mbar_wait(&bars.q_ready, 0));
-            unsigned long long t_idle = global_ns();
-            uint32_t idle = 0;
-            while (ok && pv_issued < n_kt) {
-                bool progress = false;
-                if (s_issued < n_kt && s_issued <= pv_issued + 1) {
-                    const int j = s_issued, b = j & 1;
-                    bool ready = mbar_test(&bars.k_full[b], par(j));
-                    if (ready && j >= 2) ready = mbar_test(&bars.o_full[b], par(j - 2));
-                    if (__all_sync(0xffffffffu, ready)) {
-                        tc::fence_after_sync();
-                        if (leader) {  // S(j) = (Q hi + Q lo) K^T
-                            const uint64_t k = dk + uint64_t(b) * (C::kOp >> 4);
+            auto wait_all = [](uint64_t *bar, uint32_t parity) {
+                return bool(__all_sync(0xffffffffu, mbar_wait(bar, parity)));
+            };
+            bool ok = wait_all(&bars.q_ready, 0);
+            // S(j) = (Q hi + Q lo) K^T.  Its columns hold P(j-2) until PV(j-2) is done.
+            auto issue_s = [&](int j) {
+                const int b = j & 1;
+                ok = ok && wait_all(&bars.k_full[b], par(j));
+                if (ok && j >= 2) ok = wait_all(&bars.o_full[b], par(j - 2));
+                if (!ok) return;
+                tc::fence_after_sync();
+                if (leader) {
+                    const uint64_t k = dk + uint64_t(b) * (C::kOp >> 4);
 #pragma unroll 1
-                            for (int u = 0; u < 2; ++u)
-#pragma unroll 1
-                                for (int kk = 0; kk < HD / 16; ++kk) {
-                                    const uint64_t off = ((kk >> 2) * C::kChunk + (kk & 3) * 32) >> 4;
-                                    tc::mma_f16_ss(tmem + C::kColS(b), dq + u * (C::kOp >> 4) + off, k + off,
-                                                   idesc_s, u + kk > 0 ? 1u : 0u);
-                                }
-                            tc::commit(&bars.s_full[b]);
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int kk = 0; kk < HD / 16; ++kk) {
+                            const uint64_t off = ((kk >> 2) * C::kChunk + (kk & 3) * 32) >> 4;
+                            tc::mma_f16_ss(tmem + C::kColS(b), dq + u * (C::kOp >> 4) + off, k + off, idesc_s,
+                                           u + kk > 0 ? 1u : 0u);
                         }
-                        __syncwarp();
-                        ++s_issued;
-                        progress = true;
-                    }
+                    tc::commit(&bars.s_full[b]);
                 }
-                if (pv_issued < s_issued) {
-                    const int j = pv_issued, b = j & 1;
-                    if (__all_sync(0xffffffffu, mbar_test(&bars.p_full[b], par(j)) &&
-                                                    mbar_test(&bars.v_full[b], par(j)))) {
-                        tc::fence_after_sync();
-                        if (leader) {  // O(j) = (P hi + P lo) V, from zero
-                            const uint64_t v = dv + uint64_t(b) * (C::kOp >> 4);
-#pragma unroll 1
-                            for (int kk = 0; kk < kBN / 16; ++kk)
-#pragma unroll 1
-                                for (int u = 0; u < 2; ++u)
-                                    tc::mma_bf16_ts(tmem + C::kColO(b),
-                                                    tmem + C::kColS(b) + 16 * kk + 8 * u,
-                                                    v + uint64_t(kk * 2048 >> 4), idesc_o, u + kk > 0 ? 1u : 0u);
-                            tc::commit(&bars.o_full[b]);
-                        }
-                        __syncwarp();
-                        ++pv_issued;
-                        progress = true;
-                    }
+                __syncwarp();
+                ++s_issued;
+            };
+            // O(j) = (P hi + P lo) V, from zero.
+            auto issue_pv = [&](int j) {
+                const int b = j & 1;
+                ok = ok && wait_all(&bars.v_full[b], par(j)) && wait_all(&bars.p_full[b], par(j));
+                if (!ok) return;
+                tc::fence_after_sync();
+                if (leader) {
+                    const uint64_t v = dv + uint64_t(b) * (C::kOp >> 4);
+#pragma unroll
+                    for (int kk = 0; kk < kBN / 16; ++kk)
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+                            tc::mma_bf16_ts(tmem + C::kColO(b), tmem + C::kColS(b) + 16 * kk + 8 * u,
+                                            v + uint64_t(kk * 2048 >> 4), idesc_o, u + kk > 0 ? 1u : 0u);
+                    tc::commit(&bars.o_full[b]);
                 }
-                if (progress) {
-                    idle = 0;
-                } else if ((++idle & 255) == 0) {
-                    const unsigned long long t = global_ns();
-                    if (idle == 256) t_idle = t;
-                    else if (t - t_idle > kMaxWaitNs || idle >= kMaxWaitPolls) ok = false;
-                }
+                __syncwarp();
+                ++pv_issued;
+            };
+            if (n_kt > 0) issue_s(0);
+            for (int j = 0; j < n_kt && ok; ++j) {
+                if (j + 1 < n_kt) issue_s(j + 1);
+                if (ok) issue_pv(j);
             }
             if (!ok && leader) atomicExch(&s_fail, 1);
             // nothing may be in flight when shared memory and TMEM go: wait

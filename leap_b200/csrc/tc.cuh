@@ -185,6 +185,17 @@ __device__ __forceinline__ void wait_ld16(float (&v)[16]) {
                  : "memory");
 }
 
+// st16u that other memory accesses may move across (volatile: it keeps its
+// place among the tcgen05 and barrier instructions).
+__device__ __forceinline__ void st16u_free(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+        "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
+        "r"(v[15]));
+}
+
 // 32-bit instruction descriptor for kind::f16 with BF16 A and B (format 1),
 // F32 accumulate, both K-major, dense (the layout of idesc_tf32).
 __host__ __device__ constexpr uint32_t idesc_bf16(int M, int N) {
