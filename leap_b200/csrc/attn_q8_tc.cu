@@ -19,14 +19,16 @@
 // Roles (16 warps; registers moved to where O lives by setmaxnreg, 200 + 200 +
 // 72 + 40 = 4 x 128):
 //   warps 0-7        softmax, two threads a row (64 keys and half of O's columns
-//                    each): S(j) from TMEM, p, hi/lo back over S in place; then
-//                    O(j-1), whose product ran meanwhile, into registers.
+//                    each): S(j) from TMEM, p, hi/lo back over S in place; O(j-1),
+//                    whose product ran meanwhile, into registers.
 //   warps 8-11       codes -> FP16 operand tiles (128-byte swizzle; V is used
 //                    N-major, so nothing is transposed), a tile ahead in
 //                    registers, and the tile's scales.
 //   warp 12          issues the products: S(j+1) = Q K^T, then O(j) = P V.
-// TMEM: two buffers each of S/P and O (2 x (128 + HD) columns).  Shared memory:
-// Q hi/lo, two buffers each of K and V.
+// TMEM: two buffers of S/P (128 columns each), O (HD) and Q hi/lo (HD): both
+// products take their A operand from TMEM, since two operands in shared memory
+// would fill its 128 bytes a cycle and starve everything else.  Shared memory:
+// two buffers each of K and V, and Q on its way to TMEM.
 // Long ranges are split over blocks when a launch has few tiles; partials are
 // joined by a second kernel.
 #include <algorithm>
@@ -51,11 +53,13 @@ template <int HD>
 struct Tc {
     static constexpr uint32_t kOp = kBN * HD * 2;           // one operand tile
     static constexpr uint32_t kChunk = 128 * 128;           // 64 dims of 128 rows
-    static constexpr uint32_t kQ = 0, kK = 2 * kOp, kV = 4 * kOp;
-    static constexpr size_t kSmem = 6 * size_t(kOp) + 1024;
+    static constexpr uint32_t kK = 0, kV = 2 * kOp, kQ = 4 * kOp;
+    static constexpr uint32_t kQRow = HD * 2 + 16;          // a staged query row, hi or lo
+    static constexpr size_t kSmem = 4 * size_t(kOp) + 2 * kBM * kQRow + 1024;
     static constexpr uint32_t kCols = 512;                  // TMEM columns (a power of two)
     static constexpr uint32_t kColS(int b) { return b * 128; }
-    static constexpr uint32_t kColO(int b) { return 256 + b * HD; }
+    static constexpr uint32_t kColO = 256;
+    static constexpr uint32_t kColQ(int u) { return 384 + u * (HD / 2); }
 };
 
 struct TcArgs {
@@ -69,7 +73,7 @@ struct TcArgs {
 };
 
 struct TcBars {
-    uint64_t q_ready;    // Q in shared memory (8 softmax warps)
+    uint64_t q_ready;    // Q in TMEM (8 softmax warps)
     uint64_t k_full[2], v_full[2];  // operand tile in place (4 converter warps)
     uint64_t sc_full[kSlots];       // scales of a tile in place (4 converter warps)
     uint64_t s_full[2];  // S(j) done: K buffer free (commit)
@@ -238,25 +242,45 @@ q8_tc_kernel(const TcArgs a, const __grid_constant__ Q8Seqs tab, const __grid_co
                     // largest value to [2^14, 2^15); an infinite or NaN query gives NaN
                     const int ex = min(max(int(__reduce_max_sync(0xffffffffu, __float_as_uint(top)) >> 23), 15), 254);
                     const float up = __uint_as_float(uint32_t(268 - ex) << 23);
-                    // dims 64-127 in the converters' order: neighbouring granules swapped
-                    const uint32_t off = tc::sw128_offset_b16(r, E * lane, kBM) ^ (E * lane >= 64 ? 16u : 0u);
+                    unsigned char *qs = base + C::kQ + r * C::kQRow + E * lane * 2;
 #pragma unroll
                     for (int e = 0; e < E; e += 2) {
                         const float y0 = x[u][e] * up, y1 = x[u][e + 1] * up;
                         const __half2 hi = __floats2half2_rn(y0, y1);
                         const float2 back = __half22float2(hi);
-                        *reinterpret_cast<__half2 *>(base + C::kQ + off + 2 * e) = hi;
-                        *reinterpret_cast<__half2 *>(base + C::kQ + C::kOp + off + 2 * e) =
+                        *reinterpret_cast<__half2 *>(qs + 2 * e) = hi;
+                        *reinterpret_cast<__half2 *>(qs + kBM * C::kQRow + 2 * e) =
                             __floats2half2_rn(y0 - back.x, y1 - back.y);
                     }
                     if (lane == 0) s_fac[r] = __uint_as_float(uint32_t(ex - 14) << 23) * a.scale_log2;
                 }
             }
         }
-        fence_proxy_async_smem();  // Q -> visible to the tensor core
+        // The staged rows into TMEM, a thread its row's half of the dims; dims
+        // 64-127 in the converters' order (neighbouring 8-dim granules swapped).
+        bool ok = group_and(true);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+            for (int c = 0; c < HD / 64; ++c) {  // 32 dims: 16 columns
+                uint32_t w[16];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int gr = half * (HD / 16) + 4 * c + i;
+                    const uint4 x = *reinterpret_cast<const uint4 *>(
+                        base + C::kQ + (u * kBM + row) * C::kQRow + 16 * (gr < 8 ? gr : gr ^ 1));
+                    w[4 * i] = x.x;
+                    w[4 * i + 1] = x.y;
+                    w[4 * i + 2] = x.z;
+                    w[4 * i + 3] = x.w;
+                }
+                tc::st16u(tmem + lane_off + C::kColQ(u) + half * (HD / 4) + 16 * c, w);
+            }
+        }
+        tc::wait_st();
+        tc::fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars.q_ready);
-        bool ok = __all_sync(0xffffffffu, mbar_wait(&bars.q_ready, 0));  // s_fac of every row
 
         // What this row sees: keys below `lim`, or (TREE) keys below pos and
         // those of the run whose bit is set (itself and its ancestors).
@@ -293,36 +317,38 @@ q8_tc_kernel(const TcArgs a, const __grid_constant__ Q8Seqs tab, const __grid_co
         for (int i = 0; i < OC; ++i) o[i] = 0.f;
 
         // o = o * alpha + O(j) * vdown, in FP32; most tiles move no row's maximum
-        auto absorb = [&](int j, float alpha, float vdown) -> bool {
+        auto absorb = [&](int j, float alpha, float vdown, float (&x)[4][16]) -> bool {
             const bool there = __all_sync(0xffffffffu, mbar_wait(&bars.o_full[j & 1], par(j)));
             if (!there) return false;
             tc::fence_after_sync();
-            const uint32_t ocol = tmem + lane_off + C::kColO(j & 1) + half * OC;
+            const uint32_t ocol = tmem + lane_off + C::kColO + half * OC;
             const float2 al2 = make_float2(alpha, alpha), vd2 = make_float2(vdown, vdown);
-            auto add = [&](auto still) {
-                float x[2][16];
-                tc::ld16_async(ocol, x[0]);
 #pragma unroll
-                for (int c = 0; c < OC / 16; ++c) {
-                    float(&y)[16] = x[c & 1];
-                    tc::wait_ld16(y);
-                    if (c + 1 < OC / 16) tc::ld16_async(ocol + 16 * (c + 1), x[(c + 1) & 1]);
+            for (int c = 0; c < OC / 16; ++c) tc::ld16_async(ocol + 16 * c, x[c]);
+            if (!__all_sync(0xffffffffu, alpha == 1.f)) {
 #pragma unroll
-                    for (int i = 0; i < 16; i += 2) {
-                        float2 z = make_float2(o[16 * c + i], o[16 * c + i + 1]);
-                        if (!decltype(still)::value) z = __fmul2_rn(z, al2);
-                        z = __ffma2_rn(make_float2(y[i], y[i + 1]), vd2, z);
-                        o[16 * c + i] = z.x;
-                        o[16 * c + i + 1] = z.y;
-                    }
+                for (int i = 0; i < OC; i += 2) {
+                    const float2 z = __fmul2_rn(make_float2(o[i], o[i + 1]), al2);
+                    o[i] = z.x;
+                    o[i + 1] = z.y;
                 }
-            };
-            if (__all_sync(0xffffffffu, alpha == 1.f)) add(std::true_type());
-            else add(std::false_type());
+            }
+#pragma unroll
+            for (int c = 0; c < OC / 16; ++c) {
+                tc::wait_ld16(x[c]);
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                    const float2 z = __ffma2_rn(make_float2(x[c][i], x[c][i + 1]), vd2,
+                                                make_float2(o[16 * c + i], o[16 * c + i + 1]));
+                    o[16 * c + i] = z.x;
+                    o[16 * c + i + 1] = z.y;
+                }
+            }
             return true;
         };
 
         float alpha = 1.f, vdown = 0.f;      // of the tile whose O is still to come
+        float s[4][16];                      // scores, weights, then a part of O
         for (int j = 0; j < n_kt; ++j) {
             const int b = j & 1, slot = j & (kSlots - 1);
             ok = ok && mbar_wait(&bars.sc_full[slot], uint32_t(j / kSlots) & 1u) &&
@@ -336,7 +362,6 @@ q8_tc_kernel(const TcArgs a, const __grid_constant__ Q8Seqs tab, const __grid_co
             const bool full = __all_sync(0xffffffffu, (TREE ? pos : lim) >= k0 + 64);
             const uint2 vis = full ? make_uint2(~0u, ~0u) : make_uint2(seen(k0), seen(k0 + 32));
             // scores in units of 1/fac, and the largest of the thread's half
-            float s[4][16];
             float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
             for (int c = 0; c < 4; ++c) tc::ld16_async(scol + 16 * c, s[c]);
@@ -424,16 +449,15 @@ q8_tc_kernel(const TcArgs a, const __grid_constant__ Q8Seqs tab, const __grid_co
             l = l * al + ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
             const float vd = s_vdown[slot];
             tc::wait_st();
+            // O(j-1), whose product ran beside this softmax; then PV(j) may start
+            if (j > 0) ok = absorb(j - 1, alpha, vdown, s);
             tc::fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars.p_full[b]);
-            // O(j-1), whose product ran beside this softmax
-            if (j > 0) ok = absorb(j - 1, alpha, vdown);
-            tc::fence_before_sync();  // read before PV(j+1), which p_full(j+1) allows
             alpha = al;
             vdown = vd;
         }
-        if (ok && n_kt > 0) ok = absorb(n_kt - 1, alpha, vdown);
+        if (ok && n_kt > 0) ok = absorb(n_kt - 1, alpha, vdown, s);
         if (!ok && lane == 0) atomicExch(&s_fail, 1);
         s_l[half][row] = l;
         ok = group_and(ok);
@@ -560,7 +584,6 @@ q8_tc_kernel(const TcArgs a, const __grid_constant__ Q8Seqs tab, const __grid_co
             const bool leader = tc::elect_one_sync();
             constexpr uint32_t idesc_s = tc::idesc_f16(kBM, kBN, false);
             constexpr uint32_t idesc_o = tc::idesc_f16(kBM, HD, true);
-            const uint64_t dq = tc::sw128_kmajor_desc(sbase + C::kQ);
             const uint64_t dk = tc::sw128_kmajor_desc(sbase + C::kK);
             const uint64_t dv = tc::sw128_nmajor_desc(sbase + C::kV, C::kChunk);
             int s_issued = 0, pv_issued = 0;
@@ -582,8 +605,8 @@ q8_tc_kernel(const TcArgs a, const __grid_constant__ Q8Seqs tab, const __grid_co
 #pragma unroll
                         for (int kk = 0; kk < HD / 16; ++kk) {
                             const uint64_t off = ((kk >> 2) * C::kChunk + (kk & 3) * 32) >> 4;
-                            tc::mma_f16_ss(tmem + C::kColS(b), dq + u * (C::kOp >> 4) + off, k + off, idesc_s,
-                                           u + kk > 0 ? 1u : 0u);
+                            tc::mma_f16_ts(tmem + C::kColS(b), tmem + C::kColQ(u) + 8 * kk, k + off, idesc_s,
+                                            u + kk > 0 ? 1u : 0u);
                         }
                     tc::commit(&bars.s_full[b]);
                 }
@@ -602,7 +625,7 @@ q8_tc_kernel(const TcArgs a, const __grid_constant__ Q8Seqs tab, const __grid_co
                     for (int kk = 0; kk < kBN / 16; ++kk)
 #pragma unroll
                         for (int u = 0; u < 2; ++u)
-                            tc::mma_bf16_ts(tmem + C::kColO(b), tmem + C::kColS(b) + 16 * kk + 8 * u,
+                            tc::mma_f16_ts(tmem + C::kColO, tmem + C::kColS(b) + 16 * kk + 8 * u,
                                             v + uint64_t(kk * 2048 >> 4), idesc_o, u + kk > 0 ? 1u : 0u);
                     tc::commit(&bars.o_full[b]);
                 }

@@ -230,16 +230,10 @@ __device__ __forceinline__ uint64_t sw128_nmajor_desc(uint32_t smem_byte_addr, u
            uint64_t((1024u >> 4) & 0x3FFFu) << 32 | uint64_t(1u) << 46 | uint64_t(2u) << 61;
 }
 
-// D[tmem] (+)= A[smem desc] . B[smem desc], kind::f16 (K = 16 per product).
-__device__ __forceinline__ void mma_f16_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+// The same instruction with FP16 operands (the descriptor says which).
+__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
                                            uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-        :
-        : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-        : "memory");
+    mma_bf16_ts(d_tmem, a_tmem, b_desc, idesc, accumulate);
 }
 
 // Two floats rounded to BF16 (nearest even) in one 32-bit word: `a` in the
