@@ -126,6 +126,19 @@ __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.al
 template <int N>
 __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
+template <int N>
+__device__ __forceinline__ void load_vec(float (&v)[N], const float *p) {
+    if constexpr (N == 4) {
+        const float4 x = *reinterpret_cast<const float4 *>(p);
+        v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+    } else if constexpr (N == 2) {
+        const float2 x = *reinterpret_cast<const float2 *>(p);
+        v[0] = x.x; v[1] = x.y;
+    } else {
+        v[0] = *p;
+    }
+}
+
 // Barrier of the 256 softmax threads (named barrier 1): true if `ok` everywhere.
 __device__ __forceinline__ bool group_and(bool ok) {
     uint32_t r;
@@ -203,26 +216,28 @@ q8_tc_kernel(const TcArgs a, const __grid_constant__ Q8Seqs tab, const __grid_co
         const uint32_t lane_off = uint32_t((warp & 3) * 32) << 16;
         // Q was written before the append kernel began, so it needs no wait
         {
-            constexpr int E = HD / 32, U = 4;
+            // 8 rows of a warp at a time, all their loads in flight at once
+            constexpr int E = HD / 32, U = 8;
+#pragma unroll 1
             for (int r0 = warp; r0 < kBM; r0 += 8 * U) {
-                float x[U][E];
-                int at[U];
+                float x[U][E], rc[U][E / 2], rs[U][E / 2];
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
                     const int r = r0 + 8 * u, t = t0 + r / G;
-                    at[u] = -1;
                     if (t < t_end) {
-                        at[u] = pos + t;
+                        int at = pos + t;
                         if (TREE) {
-                            at[u] = pos;
-                            for (int p = s_parent[t]; p >= 0; p = s_parent[p]) ++at[u];
+                            at = pos;
+                            for (int p = s_parent[t]; p >= 0; p = s_parent[p]) ++at;
                         }
                         const float *src = a.q + (size_t(tok0 + t) * a.L.n_kv * G + h * G + r % G) * HD + E * lane;
-#pragma unroll
-                        for (int e = 0; e < E; ++e) x[u][e] = src[e];
+                        const size_t c = size_t(at) * (HD / 2) + lane * (E / 2);
+                        load_vec<E>(x[u], src);
+                        load_vec<E / 2>(rc[u], a.rope_cos + c);
+                        load_vec<E / 2>(rs[u], a.rope_sin + c);
                     } else {
 #pragma unroll
-                        for (int e = 0; e < E; ++e) x[u][e] = 0.f;
+                        for (int e = 0; e < E; ++e) x[u][e] = rc[u][e / 2] = rs[u][e / 2] = 0.f;
                     }
                 }
 #pragma unroll
@@ -231,13 +246,10 @@ q8_tc_kernel(const TcArgs a, const __grid_constant__ Q8Seqs tab, const __grid_co
                     float top = 0.f;
 #pragma unroll
                     for (int e = 0; e < E; e += 2) {
-                        if (at[u] >= 0) {
-                            const size_t c = size_t(at[u]) * (HD / 2) + (E * lane + e) / 2;
-                            const float2 z = rope_pair(x[u][e], x[u][e + 1], a.rope_cos[c], a.rope_sin[c]);
-                            x[u][e] = z.x;
-                            x[u][e + 1] = z.y;
-                        }
-                        top = fmaxf(top, fmaxf(fabsf(x[u][e]), fabsf(x[u][e + 1])));
+                        const float2 z = rope_pair(x[u][e], x[u][e + 1], rc[u][e / 2], rs[u][e / 2]);
+                        x[u][e] = z.x;
+                        x[u][e + 1] = z.y;
+                        top = fmaxf(top, fmaxf(fabsf(z.x), fabsf(z.y)));
                     }
                     // largest value to [2^14, 2^15); an infinite or NaN query gives NaN
                     const int ex = min(max(int(__reduce_max_sync(0xffffffffu, __float_as_uint(top)) >> 23), 15), 254);
@@ -461,27 +473,31 @@ q8_tc_kernel(const TcArgs a, const __grid_constant__ Q8Seqs tab, const __grid_co
         if (!ok && lane == 0) atomicExch(&s_fail, 1);
         s_l[half][row] = l;
         ok = group_and(ok);
-        if (ok && tok < t_end) {
-            const float sum = s_l[0][row] + s_l[1][row];
-            float4 *dst;
-            size_t step;
-            float by = 1.f;
-            if (it.part < 0) {
-                dst = reinterpret_cast<float4 *>(a.out + (size_t(tok0 + tok) * a.L.n_kv * G + h * G + row % G) * HD);
-                step = 1;
-                by = 1.f / sum;
-            } else {
-                dst = reinterpret_cast<float4 *>(a.part_o) + size_t(it.part) * (HD / 4) * kBM + row;
-                step = kBM;
-                if (half == 0)
-                    reinterpret_cast<float2 *>(a.part_ml)[size_t(it.part) * kBM + row] = make_float2(m, sum);
-            }
-            dst += half * (OC / 4) * step;
+        if (ok && it.part >= 0 && tok < t_end) {
+            float4 *dst = reinterpret_cast<float4 *>(a.part_o) + (size_t(it.part) * (HD / 4) + half * (OC / 4)) * kBM + row;
+            if (half == 0)
+                reinterpret_cast<float2 *>(a.part_ml)[size_t(it.part) * kBM + row] = make_float2(m, s_l[0][row] + s_l[1][row]);
 #pragma unroll
-            for (int i = 0; i < OC / 4; ++i) {
-                // columns 64-127 have neighbouring 8-dim granules swapped
-                const int d4 = HD == 128 && half ? i ^ 2 : i;
-                dst[d4 * step] = make_float4(o[4 * i] * by, o[4 * i + 1] * by, o[4 * i + 2] * by, o[4 * i + 3] * by);
+            for (int i = 0; i < OC / 4; ++i)  // columns 64-127 have neighbouring 8-dim granules swapped
+                dst[(HD == 128 && half ? i ^ 2 : i) * kBM] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        }
+        if (ok && it.part < 0) {
+            // through shared memory (where Q was staged), so that a warp stores whole rows
+            constexpr int RS = HD * 4 + 16;
+            static_assert(kBM * RS <= 2 * kBM * C::kQRow, "output staging");
+            const float inv = 1.f / (s_l[0][row] + s_l[1][row]);
+#pragma unroll
+            for (int i = 0; i < OC / 4; ++i)
+                *reinterpret_cast<float4 *>(base + C::kQ + row * RS + half * OC * 4 + 16 * (HD == 128 && half ? i ^ 2 : i)) =
+                    make_float4(o[4 * i] * inv, o[4 * i + 1] * inv, o[4 * i + 2] * inv, o[4 * i + 3] * inv);
+            (void)group_and(true);
+            constexpr int LPR = HD / 4;  // lanes of a row
+#pragma unroll 4
+            for (int r = warp * (32 / LPR) + lane / LPR; r < kBM; r += 8 * (32 / LPR)) {
+                const int t = t0 + r / G;
+                if (t < t_end)
+                    *reinterpret_cast<float4 *>(a.out + (size_t(tok0 + t) * a.L.n_kv * G + h * G + r % G) * HD + 4 * (lane % LPR)) =
+                        *reinterpret_cast<const float4 *>(base + C::kQ + r * RS + 16 * (lane % LPR));
             }
         }
     } else if (warp < 12) {
