@@ -155,7 +155,7 @@ __device__ __forceinline__ bool group_and(bool ok) {
 
 template <int HD, int G, bool TREE>
 __global__ void __launch_bounds__(kThreads, 1)
-q8_tc_kernel(const TcArgs a, const __grid_constant__ Q8Seqs tab, const __grid_constant__ Q8TcPlan plan,
+q8_tc_kernel(const __grid_constant__ TcArgs a, const __grid_constant__ Q8Seqs tab, const __grid_constant__ Q8TcPlan plan,
              const __grid_constant__ Q8See<TREE> see) {
     using C = Tc<HD>;
     constexpr int BT = kBM / G;  // tokens of a block
@@ -216,57 +216,54 @@ q8_tc_kernel(const TcArgs a, const __grid_constant__ Q8Seqs tab, const __grid_co
         const uint32_t lane_off = uint32_t((warp & 3) * 32) << 16;
         // Q was written before the append kernel began, so it needs no wait
         {
-            // 8 rows of a warp at a time, all their loads in flight at once
-            constexpr int E = HD / 32, U = 8;
-#pragma unroll 1
-            for (int r0 = warp; r0 < kBM; r0 += 8 * U) {
-                float x[U][E], rc[U][E / 2], rs[U][E / 2];
+            // A warp's 16 rows with all their loads in flight at once.  Rows past
+            // the last token repeat it (no branch; what they give is not stored).
+            constexpr int E = HD / 32, U = kBM / 8;
+            float x[U][E], rc[U][E / 2], rs[U][E / 2];
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const int r = r0 + 8 * u, t = t0 + r / G;
-                    if (t < t_end) {
-                        int at = pos + t;
-                        if (TREE) {
-                            at = pos;
-                            for (int p = s_parent[t]; p >= 0; p = s_parent[p]) ++at;
-                        }
-                        const float *src = a.q + (size_t(tok0 + t) * a.L.n_kv * G + h * G + r % G) * HD + E * lane;
-                        const size_t c = size_t(at) * (HD / 2) + lane * (E / 2);
-                        load_vec<E>(x[u], src);
-                        load_vec<E / 2>(rc[u], a.rope_cos + c);
-                        load_vec<E / 2>(rs[u], a.rope_sin + c);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < E; ++e) x[u][e] = rc[u][e / 2] = rs[u][e / 2] = 0.f;
-                    }
-                }
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const int r = r0 + 8 * u;
-                    float top = 0.f;
-#pragma unroll
-                    for (int e = 0; e < E; e += 2) {
-                        const float2 z = rope_pair(x[u][e], x[u][e + 1], rc[u][e / 2], rs[u][e / 2]);
-                        x[u][e] = z.x;
-                        x[u][e + 1] = z.y;
-                        top = fmaxf(top, fmaxf(fabsf(z.x), fabsf(z.y)));
-                    }
-                    // largest value to [2^14, 2^15); an infinite or NaN query gives NaN
-                    const int ex = min(max(int(__reduce_max_sync(0xffffffffu, __float_as_uint(top)) >> 23), 15), 254);
-                    const float up = __uint_as_float(uint32_t(268 - ex) << 23);
-                    unsigned char *qs = base + C::kQ + r * C::kQRow + E * lane * 2;
-#pragma unroll
-                    for (int e = 0; e < E; e += 2) {
-                        const float y0 = x[u][e] * up, y1 = x[u][e + 1] * up;
-                        const __half2 hi = __floats2half2_rn(y0, y1);
-                        const float2 back = __half22float2(hi);
-                        *reinterpret_cast<__half2 *>(qs + 2 * e) = hi;
-                        *reinterpret_cast<__half2 *>(qs + kBM * C::kQRow + 2 * e) =
-                            __floats2half2_rn(y0 - back.x, y1 - back.y);
-                    }
-                    if (lane == 0) s_fac[r] = __uint_as_float(uint32_t(ex - 14) << 23) * a.scale_log2;
-                }
+            for (int u = 0; u < U; ++u) {
+                const int r = warp + 8 * u, t = min(t0 + r / G, t_end - 1);
+                const size_t c = size_t(pos + see.depth(tok0, t)) * (HD / 2) + lane * (E / 2);
+                load_vec<E>(x[u], a.q + (size_t(tok0 + t) * a.L.n_kv * G + h * G + r % G) * HD + E * lane);
+                load_vec<E / 2>(rc[u], a.rope_cos + c);
+                load_vec<E / 2>(rs[u], a.rope_sin + c);
             }
+            float fac_of_lane = 0.f;  // lane u: of row u
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int r = warp + 8 * u;
+                float top = 0.f;
+#pragma unroll
+                for (int e = 0; e < E; e += 2) {
+                    const float2 z = rope_pair(x[u][e], x[u][e + 1], rc[u][e / 2], rs[u][e / 2]);
+                    x[u][e] = z.x;
+                    x[u][e + 1] = z.y;
+                    top = fmaxf(top, fmaxf(fabsf(z.x), fabsf(z.y)));
+                }
+                // largest value to [2^14, 2^15); an infinite or NaN query gives NaN
+                const int ex = min(max(int(__reduce_max_sync(0xffffffffu, __float_as_uint(top)) >> 23), 15), 254);
+                const float up = __uint_as_float(uint32_t(268 - ex) << 23);
+                uint32_t hi[E / 2], lo[E / 2];
+#pragma unroll
+                for (int e = 0; e < E; e += 2) {
+                    const float y0 = x[u][e] * up, y1 = x[u][e + 1] * up;
+                    const __half2 a2 = __floats2half2_rn(y0, y1);
+                    const float2 back = __half22float2(a2);
+                    const __half2 b2 = __floats2half2_rn(y0 - back.x, y1 - back.y);
+                    hi[e / 2] = *reinterpret_cast<const uint32_t *>(&a2);
+                    lo[e / 2] = *reinterpret_cast<const uint32_t *>(&b2);
+                }
+                unsigned char *qs = base + C::kQ + r * C::kQRow + E * lane * 2;
+                if constexpr (E == 4) {
+                    *reinterpret_cast<uint2 *>(qs) = make_uint2(hi[0], hi[1]);
+                    *reinterpret_cast<uint2 *>(qs + kBM * C::kQRow) = make_uint2(lo[0], lo[1]);
+                } else {
+                    *reinterpret_cast<uint32_t *>(qs) = hi[0];
+                    *reinterpret_cast<uint32_t *>(qs + kBM * C::kQRow) = lo[0];
+                }
+                fac_of_lane = lane == u ? __uint_as_float(uint32_t(ex - 14) << 23) * a.scale_log2 : fac_of_lane;
+            }
+            if (lane < U) s_fac[warp + 8 * lane] = fac_of_lane;
         }
         // The staged rows into TMEM, a thread its row's half of the dims; dims
         // 64-127 in the converters' order (neighbouring 8-dim granules swapped).

@@ -764,7 +764,11 @@ int leap_attn_tree(leap_ctx *c, int layer, int n_seq, const int *slots, const in
         leap::Q8Tree tree;
         next_seqs(tab, n_seq, slots, positions, n_nodes, leap::kMaxNodesPerLaunch, &i);
         const int done = tab.tok0[tab.n_seq];
-        for (int j = 0; j < done; ++j) tree.parent[j] = int8_t(parents[j]);
+        for (int b = 0; b < tab.n_seq; ++b)
+            for (int j = tab.tok0[b]; j < tab.tok0[b + 1]; ++j) {
+                tree.parent[j] = int8_t(parents[j]);
+                tree.depth[j] = parents[j] < 0 ? 0 : int8_t(tree.depth[tab.tok0[b] + parents[j]] + 1);
+            }
         const int st = leap::q8_attend(c, layer, tab, &tree, q, k, v, out);
         c->last_written_layer = layer;
         if (st) return st;
@@ -802,10 +806,10 @@ int leap_kv_keep(leap_ctx *c, int n_seq, const int *slots, const int *positions,
     c->last_written_layer = leap_ctx::kWroteAll;
     for (int i = 0; i < n_seq;) {
         leap::Q8Seqs tab;
-        leap::Q8Tree keep;
+        leap::Q8Nodes keep;
         next_seqs(tab, n_seq, slots, positions, n_keep, leap::kMaxNodesPerLaunch, &i);
         const int done = tab.tok0[tab.n_seq];
-        for (int j = 0; j < done; ++j) keep.parent[j] = int8_t(nodes[j]);
+        for (int j = 0; j < done; ++j) keep.at[j] = int8_t(nodes[j]);
         if (int st = leap::kv_keep(c, tab, keep)) return st;
         nodes += done;
     }

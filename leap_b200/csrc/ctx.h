@@ -162,9 +162,13 @@ struct Q8Seqs {
     int pos[kMaxSeqPerLaunch];
     int tok0[kMaxSeqPerLaunch + 1];
 };
-// Parent of each packed token, counted from its sequence's first; -1: none.
+// Parent of each packed token, counted from its sequence's first (-1: none),
+// and its depth.
 struct Q8Tree {
-    int8_t parent[kMaxNodesPerLaunch];
+    int8_t parent[kMaxNodesPerLaunch], depth[kMaxNodesPerLaunch];
+};
+struct Q8Nodes {
+    int8_t at[kMaxNodesPerLaunch];
 };
 
 // Splits of the sequences' cached rows: `chunk` rows each, sequence i's are
@@ -204,8 +208,8 @@ int q8_read(leap_ctx *c, int slot, int layer, int pos0, int n, float *k, float *
 int q8_append(leap_ctx *c, int layer, const Q8Seqs &tab, const Q8Tree *tree, const float *k,
               const float *v);
 int kv_read_packed(leap_ctx *c, int layer, const Q8Seqs &tab, float *k, float *v);
-// Move rows pos + node[j] to pos + j (j counted from each sequence's first).
-int kv_keep(leap_ctx *c, const Q8Seqs &tab, const Q8Tree &nodes);
+// Move rows pos + at[j] to pos + j (j counted from each sequence's first).
+int kv_keep(leap_ctx *c, const Q8Seqs &tab, const Q8Nodes &nodes);
 int q8_rows_parts(const leap_ctx *c);
 int q8_rows_attend(leap_ctx *c, int layer, const Q8Seqs &tab, const Q8Tree *tree, const float *q,
                    const float *k, const float *v, float *out);

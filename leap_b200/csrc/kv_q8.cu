@@ -137,10 +137,10 @@ __device__ __forceinline__ void keep_rows(T *head, int n, int pos, const int8_t 
 template <int HD>
 __global__ void __launch_bounds__(96)
 q8_keep_kernel(const Q8Layer L, size_t layer_rows, const __grid_constant__ Q8Seqs tab,
-               const __grid_constant__ Q8Tree nodes) {
+               const __grid_constant__ Q8Nodes nodes) {
     const int seq = blockIdx.x, h = blockIdx.z;
     const int t0 = tab.tok0[seq], n = tab.tok0[seq + 1] - t0, pos = tab.pos[seq];
-    const int8_t *node = nodes.parent + t0;
+    const int8_t *node = nodes.at + t0;
     const size_t r0 = tab.slot[seq] * L.slot_rows + blockIdx.y * layer_rows + h * L.head_rows;
     const int lane = threadIdx.x & 31, what = threadIdx.x >> 5;
     using T = typename std::conditional<HD == 128, uint32_t, uint16_t>::type;
@@ -156,14 +156,14 @@ q8_keep_kernel(const Q8Layer L, size_t layer_rows, const __grid_constant__ Q8Seq
 
 __global__ void __launch_bounds__(64)
 f32_keep_kernel(float *kc, float *vc, size_t head_stride, size_t layer_stride, size_t slot_stride,
-                int hd4, const __grid_constant__ Q8Seqs tab, const __grid_constant__ Q8Tree nodes) {
+                int hd4, const __grid_constant__ Q8Seqs tab, const __grid_constant__ Q8Nodes nodes) {
     const int seq = blockIdx.x;
     const int t0 = tab.tok0[seq], n = tab.tok0[seq + 1] - t0;
     const int lane = threadIdx.x & 31;
     float *head = ((threadIdx.x >> 5) ? vc : kc) + tab.slot[seq] * slot_stride +
                   blockIdx.y * layer_stride + blockIdx.z * head_stride;
     if (lane < hd4)
-        keep_rows(reinterpret_cast<float4 *>(head), n, tab.pos[seq], nodes.parent + t0,
+        keep_rows(reinterpret_cast<float4 *>(head), n, tab.pos[seq], nodes.at + t0,
                   [lane, hd4](int r) { return size_t(r) * hd4 + lane; });
 }
 
@@ -313,7 +313,7 @@ int kv_read_packed(leap_ctx *c, int layer, const Q8Seqs &tab, float *k, float *v
     return cuda_status(cudaGetLastError(), "f32_read_kernel launch");
 }
 
-int kv_keep(leap_ctx *c, const Q8Seqs &tab, const Q8Tree &nodes) {
+int kv_keep(leap_ctx *c, const Q8Seqs &tab, const Q8Nodes &nodes) {
     const dim3 grid(tab.n_seq, c->n_layers, c->n_kv);
     if (c->kv_kind != LEAP_KV_Q8) {
         f32_keep_kernel<<<grid, 64, 0, c->stream>>>(c->k_cache, c->v_cache, c->head_stride,

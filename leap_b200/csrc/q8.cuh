@@ -56,11 +56,7 @@ template <>
 struct Q8See<true> {
     Q8Tree tree;
     // t0: the sequence's first packed token.  Parents come before children.
-    __device__ __forceinline__ int depth(int t0, int i) const {
-        int d = 0;
-        for (int p = tree.parent[t0 + i]; p >= 0; p = tree.parent[t0 + p]) ++d;
-        return d;
-    }
+    __device__ __forceinline__ int depth(int t0, int i) const { return tree.depth[t0 + i]; }
     __device__ __forceinline__ bool sees(int t0, int i, int j) const {
         while (i > j) i = tree.parent[t0 + i];
         return i == j;
