@@ -67,7 +67,7 @@ struct TcArgs {
     float *out;
     Q8Layer L;
     const float *rope_cos, *rope_sin;
-    float *part_o, *part_ml;  // [parts][HD/4][128] float4, [parts][128][2]
+    float *part_o, *part_ml;  // [parts][128][HD], [parts][128][2]
     int *err;
     float scale_log2;
 };
@@ -443,9 +443,10 @@ q8_tc_kernel(const __grid_constant__ TcArgs a, const __grid_constant__ Q8Seqs ta
                             if (off[c] >> (2 * i + 1) & 1) w.y = 0.f;
                         }
                         sum[i & 1] = __fadd2_rn(sum[i & 1], p);
-                        const __half2 hi = __floats2half2_rn(w.x, w.y);
-                        const float2 back = __half22float2(hi);
-                        const float2 r = __fadd2_rn(w, make_float2(-back.x, -back.y));
+                        // hi: the top 11 bits (exact in FP16), cheaper than to round and convert back
+                        const float2 top = make_float2(tc::tf32_hi(w.x), tc::tf32_hi(w.y));
+                        const __half2 hi = __floats2half2_rn(top.x, top.y);
+                        const float2 r = __fadd2_rn(w, make_float2(-top.x, -top.y));
                         const __half2 lo = __floats2half2_rn(r.x, r.y);
                         hl[i] = *reinterpret_cast<const uint32_t *>(&hi);
                         hl[8 + i] = *reinterpret_cast<const uint32_t *>(&lo);
@@ -470,30 +471,26 @@ q8_tc_kernel(const __grid_constant__ TcArgs a, const __grid_constant__ Q8Seqs ta
         if (!ok && lane == 0) atomicExch(&s_fail, 1);
         s_l[half][row] = l;
         ok = group_and(ok);
-        if (ok && it.part >= 0 && tok < t_end) {
-            float4 *dst = reinterpret_cast<float4 *>(a.part_o) + (size_t(it.part) * (HD / 4) + half * (OC / 4)) * kBM + row;
-            if (half == 0)
-                reinterpret_cast<float2 *>(a.part_ml)[size_t(it.part) * kBM + row] = make_float2(m, s_l[0][row] + s_l[1][row]);
-#pragma unroll
-            for (int i = 0; i < OC / 4; ++i)  // columns 64-127 have neighbouring 8-dim granules swapped
-                dst[(HD == 128 && half ? i ^ 2 : i) * kBM] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-        }
-        if (ok && it.part < 0) {
+        if (ok) {
             // through shared memory (where Q was staged), so that a warp stores whole rows
             constexpr int RS = HD * 4 + 16;
             static_assert(kBM * RS <= 2 * kBM * C::kQRow, "output staging");
-            const float inv = 1.f / (s_l[0][row] + s_l[1][row]);
+            const float sum = s_l[0][row] + s_l[1][row], by = it.part < 0 ? 1.f / sum : 1.f;
+            if (it.part >= 0 && half == 0 && tok < t_end)
+                reinterpret_cast<float2 *>(a.part_ml)[size_t(it.part) * kBM + row] = make_float2(m, sum);
 #pragma unroll
-            for (int i = 0; i < OC / 4; ++i)
+            for (int i = 0; i < OC / 4; ++i)  // columns 64-127 have neighbouring 8-dim granules swapped
                 *reinterpret_cast<float4 *>(base + C::kQ + row * RS + half * OC * 4 + 16 * (HD == 128 && half ? i ^ 2 : i)) =
-                    make_float4(o[4 * i] * inv, o[4 * i + 1] * inv, o[4 * i + 2] * inv, o[4 * i + 3] * inv);
+                    make_float4(o[4 * i] * by, o[4 * i + 1] * by, o[4 * i + 2] * by, o[4 * i + 3] * by);
             (void)group_and(true);
             constexpr int LPR = HD / 4;  // lanes of a row
 #pragma unroll 4
             for (int r = warp * (32 / LPR) + lane / LPR; r < kBM; r += 8 * (32 / LPR)) {
                 const int t = t0 + r / G;
+                float *dst = it.part < 0 ? a.out + (size_t(tok0 + t) * a.L.n_kv * G + h * G + r % G) * HD
+                                         : a.part_o + (size_t(it.part) * kBM + r) * HD;
                 if (t < t_end)
-                    *reinterpret_cast<float4 *>(a.out + (size_t(tok0 + t) * a.L.n_kv * G + h * G + r % G) * HD + 4 * (lane % LPR)) =
+                    *reinterpret_cast<float4 *>(dst + 4 * (lane % LPR)) =
                         *reinterpret_cast<const float4 *>(base + C::kQ + r * RS + 16 * (lane % LPR));
             }
         }
@@ -691,7 +688,7 @@ q8_tc_join_kernel(const TcArgs a, const __grid_constant__ Q8Seqs tab, const __gr
     if (tok >= tab.tok0[seq + 1] - tok0) return;
     const size_t p0 = size_t(plan.part0[lo] + i * ns) * n_kv + h;  // splits n_kv apart
     const float2 *ml = reinterpret_cast<const float2 *>(a.part_ml) + p0 * kBM + row;
-    const float4 *po = reinterpret_cast<const float4 *>(a.part_o) + p0 * (HD / 4) * kBM + row;
+    const float4 *po = reinterpret_cast<const float4 *>(a.part_o) + (p0 * kBM + row) * (HD / 4) + lane;
     float mx = -INFINITY;
     for (int s = lane; s < ns; s += 32) mx = fmaxf(mx, ml[size_t(s) * n_kv * kBM].x);
 #pragma unroll
@@ -701,7 +698,7 @@ q8_tc_join_kernel(const TcArgs a, const __grid_constant__ Q8Seqs tab, const __gr
 #pragma unroll 4
     for (int s = 0; s < ns; ++s) {
         const float2 y = ml[size_t(s) * n_kv * kBM];
-        const float4 z = lane < HD / 4 ? po[size_t(s) * n_kv * (HD / 4) * kBM + size_t(lane) * kBM]
+        const float4 z = lane < HD / 4 ? po[size_t(s) * n_kv * kBM * (HD / 4)]
                                        : make_float4(0.f, 0.f, 0.f, 0.f);
         if (y.x == -INFINITY) continue;  // the split had nothing this row sees
         const float e = fast_exp2(y.x - mx);
