@@ -126,19 +126,6 @@ __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.al
 template <int N>
 __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
-template <int N>
-__device__ __forceinline__ void load_vec(float (&v)[N], const float *p) {
-    if constexpr (N == 4) {
-        const float4 x = *reinterpret_cast<const float4 *>(p);
-        v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-    } else if constexpr (N == 2) {
-        const float2 x = *reinterpret_cast<const float2 *>(p);
-        v[0] = x.x; v[1] = x.y;
-    } else {
-        v[0] = *p;
-    }
-}
-
 // Barrier of the 256 softmax threads (named barrier 1): true if `ok` everywhere.
 __device__ __forceinline__ bool group_and(bool ok) {
     uint32_t r;

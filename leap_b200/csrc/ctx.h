@@ -171,11 +171,18 @@ struct Q8Nodes {
     int8_t at[kMaxNodesPerLaunch];
 };
 
-// Splits of the sequences' cached rows: `chunk` rows each, sequence i's are
-// split0[i] .. split0[i+1]-1 (none for a sequence without new tokens).
+// Splits of the rows kernel: `chunk` cached rows each, sequence i's are split0[i]
+// .. split0[i+1]-1 (none without new tokens).
 struct Q8Splits {
     int chunk;
     int split0[kMaxSeqPerLaunch + 1];
+};
+// The warps kernel's work list: sequence i has units unit0[i] .. unit0[i+1]-1
+// (tiles of 32 rows, kv head by kv head; none without new tokens), a warp `chunk`
+// of them.
+struct Q8Units {
+    int chunk;
+    int unit0[kMaxSeqPerLaunch + 1];
 };
 // Blocks of the tensor-core kernel: entry i is sequence seq[i] (those without
 // tokens left out, longest first), n_qt[i] query tiles of 128 rows, each over
@@ -211,6 +218,7 @@ int kv_read_packed(leap_ctx *c, int layer, const Q8Seqs &tab, float *k, float *v
 // Move rows pos + at[j] to pos + j (j counted from each sequence's first).
 int kv_keep(leap_ctx *c, const Q8Seqs &tab, const Q8Nodes &nodes);
 int q8_rows_parts(const leap_ctx *c);
+int q8_warps_parts(const leap_ctx *c);
 int q8_rows_attend(leap_ctx *c, int layer, const Q8Seqs &tab, const Q8Tree *tree, const float *q,
                    const float *k, const float *v, float *out);
 // The run's rows are stored already.

@@ -8,6 +8,8 @@
 // and each row is stored as one 128-byte (or 64-byte) line.  Nothing is staged
 // in shared memory; with 8 warps a block and 8 blocks an SM, 64 KB of loads
 // are in flight on each SM.
+#include <algorithm>
+
 #include "q8.cuh"
 
 namespace leap {
@@ -222,7 +224,7 @@ int q8_create(leap_ctx *c) {
     if (e == cudaSuccess) e = cudaMalloc(&c->ks8, rows * sizeof(float));
     if (e == cudaSuccess) e = cudaMalloc(&c->vs8, rows * sizeof(float));
     if (e == cudaSuccess) e = cudaMalloc(&c->d_rows, stage);
-    c->q8_parts = q8_rows_parts(c);
+    c->q8_parts = std::max(q8_rows_parts(c), q8_warps_parts(c));
     const size_t part = size_t(c->q8_parts) * kQ8Rows * sizeof(float);
     const size_t cnt = size_t(kMaxSeqPerLaunch) * c->n_kv * sizeof(unsigned);
     if (e == cudaSuccess) e = cudaMalloc(&c->q8_part_o, part * c->hd);

@@ -23,6 +23,19 @@
 
 namespace leap {
 
+template <int N>
+__device__ __forceinline__ void load_vec(float (&v)[N], const float *p) {
+    if constexpr (N == 4) {
+        const float4 x = *reinterpret_cast<const float4 *>(p);
+        v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+    } else if constexpr (N == 2) {
+        const float2 x = *reinterpret_cast<const float2 *>(p);
+        v[0] = x.x; v[1] = x.y;
+    } else {
+        v[0] = *p;
+    }
+}
+
 // Byte offset, from the first row of a head, of 16-byte chunk `c` of row `r`.
 template <int HD>
 __host__ __device__ __forceinline__ size_t q8_chunk(int r, int c) {
