@@ -2,12 +2,10 @@
 // without the rotation), read back, and the compaction after a verified tree.
 //
 // All of it is bound by HBM: a row of K and V of one kv head is 8*HD bytes of
-// FP32 on one side and 2*(HD + 4) bytes on the other.  One warp takes one
-// (token, kv head): a lane holds HD/32 neighbouring dims of k and of v (a
+// FP32 on one side and 2*(HD + 4) bytes on the other.  One warp takes two
+// (token, kv head) pairs, all their loads in flight together: a lane holds HD/32 neighbouring dims of k and of v (a
 // rotation pair never leaves a lane), the row's maximum is one warp reduction,
-// and each row is stored as one 128-byte (or 64-byte) line.  Nothing is staged
-// in shared memory; with 8 warps a block and 8 blocks an SM, 64 KB of loads
-// are in flight on each SM.
+// and each row is stored as one 128-byte (or 64-byte) line.
 #include <algorithm>
 
 #include "q8.cuh"
@@ -16,6 +14,7 @@ namespace leap {
 namespace {
 
 constexpr int kWarps = 8;  // warps of a block
+constexpr int kItems = 2;  // (token, kv head) pairs of a warp
 
 enum { kRaw = 0, kCausal = 1, kTree = 2 };  // what the append kernel rotates by
 
@@ -28,76 +27,89 @@ template <> struct Vec<64> { using T = float2; };
 // kTree: k rotated for position pos + depth.
 template <int HD, int MODE>
 __global__ void __launch_bounds__(32 * kWarps)
-q8_append_kernel(const float *__restrict__ k, const float *__restrict__ v, const Q8Layer L,
+q8_append_kernel(const float *__restrict__ k, const float *__restrict__ v, const __grid_constant__ Q8Layer L,
                  const float *__restrict__ rope_cos, const float *__restrict__ rope_sin,
                  const __grid_constant__ Q8Seqs tab,
                  const __grid_constant__ Q8See<MODE == kTree> see) {
     constexpr int E = HD / 32;
     grid_launch_dependents();  // what follows waits for this grid before it reads
     const int lane = threadIdx.x & 31;
-    const int item = blockIdx.x * kWarps + (threadIdx.x >> 5);
-    const int total = tab.tok0[tab.n_seq];
-    if (item >= total * L.n_kv) return;
-    const int t = item / L.n_kv, h = item - t * L.n_kv;
-    const int seq = q8_seq_of(tab, t);
-    const int i = t - tab.tok0[seq];
-    const int row = tab.pos[seq] + i;
-    using V = typename Vec<HD>::T;
-    const V kx = *reinterpret_cast<const V *>(k + size_t(item) * HD + E * lane);
-    const V vx = *reinterpret_cast<const V *>(v + size_t(item) * HD + E * lane);
-    float x[E], y[E];
+    const int first = (blockIdx.x * kWarps + (threadIdx.x >> 5)) * kItems;
+    const int items = tab.tok0[tab.n_seq] * L.n_kv;
+    float x[kItems][E], y[kItems][E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        x[e] = reinterpret_cast<const float *>(&kx)[e];
-        y[e] = reinterpret_cast<const float *>(&vx)[e];
-    }
-    if (MODE != kRaw) {
-        const int at = tab.pos[seq] + see.depth(tab.tok0[seq], i);
-        const float *rc = rope_cos + size_t(at) * (HD / 2) + lane * (E / 2);
-        const float *rs = rope_sin + size_t(at) * (HD / 2) + lane * (E / 2);
-#pragma unroll
-        for (int e = 0; e < E; e += 2) {
-            const float2 r = rope_pair(x[e], x[e + 1], rc[e / 2], rs[e / 2]);
-            x[e] = r.x;
-            x[e + 1] = r.y;
+    for (int u = 0; u < kItems; ++u)
+        if (first + u < items) {
+            load_vec<E>(x[u], k + size_t(first + u) * HD + E * lane);
+            load_vec<E>(y[u], v + size_t(first + u) * HD + E * lane);
         }
-    }
-    const size_t r0 = tab.slot[seq] * L.slot_rows + h * L.head_rows;
-    uint32_t c;
-    const float sk = q8_quantize<E>(x, c);
-    q8_store_codes<HD>(L.k + r0 * HD, row, lane, c);
-    const float sv = q8_quantize<E>(y, c);
-    q8_store_codes<HD>(L.v + r0 * HD, row, lane, c);
-    if (lane == 0) {
-        L.ks[r0 + row] = sk;
-        L.vs[r0 + row] = sv;
+#pragma unroll
+    for (int u = 0; u < kItems; ++u) {
+        if (first + u >= items) return;
+        const int t = (first + u) / L.n_kv, h = first + u - t * L.n_kv;
+        const int seq = q8_seq_of(tab, t);
+        const int i = t - tab.tok0[seq];
+        const int row = tab.pos[seq] + i;
+        if (MODE != kRaw) {
+            const size_t c = size_t(tab.pos[seq] + see.depth(tab.tok0[seq], i)) * (HD / 2) + lane * (E / 2);
+            float rc[E / 2], rs[E / 2];
+            load_vec<E / 2>(rc, rope_cos + c);
+            load_vec<E / 2>(rs, rope_sin + c);
+#pragma unroll
+            for (int e = 0; e < E; e += 2) {
+                const float2 r = rope_pair(x[u][e], x[u][e + 1], rc[e / 2], rs[e / 2]);
+                x[u][e] = r.x;
+                x[u][e + 1] = r.y;
+            }
+        }
+        const size_t r0 = tab.slot[seq] * L.slot_rows + h * L.head_rows;
+        uint32_t c;
+        const float sk = q8_quantize<E>(x[u], c);
+        q8_store_codes<HD>(L.k + r0 * HD, row, lane, c);
+        const float sv = q8_quantize<E>(y[u], c);
+        q8_store_codes<HD>(L.v + r0 * HD, row, lane, c);
+        if (lane == 0) {
+            L.ks[r0 + row] = sk;
+            L.vs[r0 + row] = sv;
+        }
     }
 }
 
 template <int HD>
 __global__ void __launch_bounds__(32 * kWarps)
-q8_read_kernel(float *__restrict__ k, float *__restrict__ v, const Q8Layer L,
+q8_read_kernel(float *__restrict__ k, float *__restrict__ v, const __grid_constant__ Q8Layer L,
                const __grid_constant__ Q8Seqs tab) {
     constexpr int E = HD / 32;
     const int lane = threadIdx.x & 31;
-    const int item = blockIdx.x * kWarps + (threadIdx.x >> 5);
-    if (item >= tab.tok0[tab.n_seq] * L.n_kv) return;
-    const int t = item / L.n_kv, h = item - t * L.n_kv;
-    const int seq = q8_seq_of(tab, t);
-    const int row = tab.pos[seq] + t - tab.tok0[seq];
-    const size_t r0 = tab.slot[seq] * L.slot_rows + h * L.head_rows;
-    const uint32_t ck = q8_load_codes<HD>(L.k + r0 * HD, row, lane);
-    const uint32_t cv = q8_load_codes<HD>(L.v + r0 * HD, row, lane);
-    const float sk = L.ks[r0 + row], sv = L.vs[r0 + row];
-    using V = typename Vec<HD>::T;
-    V x, y;
+    const int first = (blockIdx.x * kWarps + (threadIdx.x >> 5)) * kItems;
+    const int items = tab.tok0[tab.n_seq] * L.n_kv;
+    uint32_t ck[kItems], cv[kItems];
+    float sk[kItems], sv[kItems];
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        reinterpret_cast<float *>(&x)[e] = float(int((ck >> (8 * e)) & 255u) - 128) * sk;
-        reinterpret_cast<float *>(&y)[e] = float(int((cv >> (8 * e)) & 255u) - 128) * sv;
+    for (int u = 0; u < kItems; ++u)
+        if (first + u < items) {
+            const int t = (first + u) / L.n_kv, h = first + u - t * L.n_kv;
+            const int seq = q8_seq_of(tab, t);
+            const int row = tab.pos[seq] + t - tab.tok0[seq];
+            const size_t r0 = tab.slot[seq] * L.slot_rows + h * L.head_rows;
+            ck[u] = q8_load_codes<HD>(L.k + r0 * HD, row, lane);
+            cv[u] = q8_load_codes<HD>(L.v + r0 * HD, row, lane);
+            sk[u] = L.ks[r0 + row];
+            sv[u] = L.vs[r0 + row];
+        }
+    using V = typename Vec<HD>::T;
+#pragma unroll
+    for (int u = 0; u < kItems; ++u) {
+        if (first + u >= items) return;
+        V x, y;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            reinterpret_cast<float *>(&x)[e] = float(int((ck[u] >> (8 * e)) & 255u) - 128) * sk[u];
+            reinterpret_cast<float *>(&y)[e] = float(int((cv[u] >> (8 * e)) & 255u) - 128) * sv[u];
+        }
+        *reinterpret_cast<V *>(k + size_t(first + u) * HD + E * lane) = x;
+        *reinterpret_cast<V *>(v + size_t(first + u) * HD + E * lane) = y;
     }
-    *reinterpret_cast<V *>(k + size_t(item) * HD + E * lane) = x;
-    *reinterpret_cast<V *>(v + size_t(item) * HD + E * lane) = y;
 }
 
 // The same from an FP32 cache.
@@ -174,7 +186,7 @@ int launch_append(leap_ctx *c, int layer, const Q8Seqs &tab, const Q8See<MODE ==
                   const float *k, const float *v) {
     const int items = tab.tok0[tab.n_seq] * c->n_kv;
     if (items == 0) return LEAP_OK;
-    q8_append_kernel<HD, MODE><<<(items + kWarps - 1) / kWarps, 32 * kWarps, 0, c->stream>>>(
+    q8_append_kernel<HD, MODE><<<(items + kWarps * kItems - 1) / (kWarps * kItems), 32 * kWarps, 0, c->stream>>>(
         k, v, q8_layer(c, layer), c->rope_cos, c->rope_sin, tab, see);
     return cuda_status(cudaGetLastError(), "q8_append_kernel launch");
 }
@@ -182,7 +194,7 @@ int launch_append(leap_ctx *c, int layer, const Q8Seqs &tab, const Q8See<MODE ==
 int launch_read(leap_ctx *c, int layer, const Q8Seqs &tab, float *k, float *v) {
     const int items = tab.tok0[tab.n_seq] * c->n_kv;
     if (items == 0) return LEAP_OK;
-    const int grid = (items + kWarps - 1) / kWarps;
+    const int grid = (items + kWarps * kItems - 1) / (kWarps * kItems);
     if (c->hd == 128)
         q8_read_kernel<128><<<grid, 32 * kWarps, 0, c->stream>>>(k, v, q8_layer(c, layer), tab);
     else

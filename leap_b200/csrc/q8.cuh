@@ -91,25 +91,50 @@ __device__ __forceinline__ int q8_code(float x, float s, float inv) {
     return int(fminf(fmaxf(q, -127.f), 127.f));
 }
 
+// The larger of a and |b|; NaN if either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(fabsf(b)));
+    return d;
+}
+
 // One warp quantises one row, lane l holding x[E] = dims E*l .. E*l+E-1.
 // Returns the scale (the same in every lane) and this lane's codes + 128, the
 // lowest dim in the lowest byte.
 template <int E>
 __device__ __forceinline__ float q8_quantize(const float (&x)[E], uint32_t &codes) {
-    uint32_t top = 0;
+    float most = 0.f;
 #pragma unroll
-    for (int i = 0; i < E; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
-    top = __reduce_max_sync(0xffffffffu, top);
+    for (int i = 0; i < E; ++i) most = max_nan(most, x[i]);
+    const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
     codes = E == 4 ? 0x80808080u : 0x8080u;
     if (top >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
     const float s = __fmul_rn(__uint_as_float(top), 1.0f / 127.0f);
     if (s == 0.f) return 0.f;
     // tiny rows: x and s by 2^64 (exact), so that 1/s stays finite
-    const float up = top < 0x21800000u /* 2^-60 */ ? 18446744073709551616.f : 1.f;
-    const float su = s * up, inv = 1.0f / su;
-    codes = 0;
+    const bool tiny = top < 0x21800000u;  // 2^-60
+    const float up = tiny ? 18446744073709551616.f : 1.f, su = s * up, inv = 1.0f / su;
+    // x*inv + 128 + 1.5*2^23 has the rounded sum's integer in its low bits.  Where no
+    // residual reaches half a step this is the code: |x| <= 127.5 s then, unless s has
+    // lost bits (tiny).  Instructions bound the append, and the exact test of every
+    // value takes three times as many.
+    constexpr float kMagic = 12582912.f + 128.f;
+    float off = 0.f;
+    uint32_t t[E];
 #pragma unroll
-    for (int i = 0; i < E; ++i) codes |= uint32_t(q8_code(x[i] * up, su, inv) + 128) << (8 * i);
+    for (int i = 0; i < E; ++i) {
+        const float m = fmaf(x[i] * up, inv, kMagic);
+        off = fmaxf(off, fabsf(fmaf(kMagic - m, su, x[i] * up)));
+        t[i] = __float_as_uint(m);
+    }
+    if (off < 0.5f * su && !tiny) {
+        if constexpr (E == 4) codes = __byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410);
+        else codes = __byte_perm(t[0], t[1], 0x0040) & 0xffffu;
+    } else {
+        codes = 0;
+#pragma unroll
+        for (int i = 0; i < E; ++i) codes |= uint32_t(q8_code(x[i] * up, su, inv) + 128) << (8 * i);
+    }
     return s;
 }
 
