@@ -77,11 +77,10 @@ SIGNATURES: dict[str, tuple] = {
                                  c_void_p]),
     "leap_attn_decode_host": (c_int, [c_void_p, c_int, c_int, c_void_p, c_void_p,
                                       c_void_p, c_void_p]),
-    "leap_attn_decode_batched": (c_int, [c_void_p, c_int, c_int, c_int_p, c_int_p,
-                                         c_void_p, c_void_p, c_void_p, c_void_p]),
+    # the ragged calls take their host int arrays as addresses
+    "leap_attn_decode_batched": (c_int, [c_void_p, c_int, c_int] + [c_void_p] * 6),
     "leap_attn_prefill": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_void_p,
                                   c_void_p, c_void_p, c_void_p]),
-    # the ragged calls take their host int arrays as addresses
     "leap_attn_prefill_packed": (c_int, [c_void_p, c_int, c_int] + [c_void_p] * 7),
     "leap_attn_tree": (c_int, [c_void_p, c_int, c_int] + [c_void_p] * 8),
     "leap_kv_keep": (c_int, [c_void_p, c_int] + [c_void_p] * 4),
@@ -155,6 +154,8 @@ class LeapError(RuntimeError):
 
 def lib() -> ctypes.CDLL:
     global _lib
+    if _lib is not None:  # set once, complete
+        return _lib
     with _lock:
         if _lib is None:
             if not os.path.exists(LIB_PATH):

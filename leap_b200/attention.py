@@ -33,9 +33,15 @@ def rope_table(seq_len: int, head_dim: int, theta: float = 500000.0):
     return c, s
 
 
+_torch = None  # imported with the first device tensor
+
+
 def _dptr(t) -> int:
     """Device pointer of a contiguous float32 CUDA tensor."""
-    import torch
+    global _torch
+    if _torch is None:
+        import torch as _torch
+    torch = _torch
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise TypeError("expected a CUDA torch.Tensor")
     if t.dtype != torch.float32 or not t.is_contiguous():
@@ -58,6 +64,17 @@ def _ints(a, name: str, n: int | None = None) -> np.ndarray:
     if a.ndim != 1 or (n is not None and a.shape[0] != n):
         raise ValueError(f"{name} must be 1-D" + ("" if n is None else f" of length {n}"))
     return a
+
+
+def _iptr(a: np.ndarray) -> int:
+    """Address of a contiguous host array (cheaper than ``a.ctypes.data``)."""
+    return a.__array_interface__["data"][0]
+
+
+def _total(a: np.ndarray) -> int:
+    """Sum of the lengths (negative ones, which the library refuses, as 0)."""
+    t = a.tolist()
+    return sum(t) if not t or min(t) >= 0 else sum(x for x in t if x > 0)
 
 
 def _hptr(a: np.ndarray) -> int:
@@ -186,9 +203,9 @@ class AttentionContext:
         slots = _ints(slots, "slots")
         n = slots.shape[0]
         pos0, n_tok = _ints(pos0, "pos0", n), _ints(n_tok, "n_tok", n)
-        k, v = self._rows(int(n_tok.clip(0).sum()))
-        check(lib().leap_kv_read_packed(self.handle, layer, n, slots.ctypes.data,
-                                        pos0.ctypes.data, n_tok.ctypes.data, k.data_ptr(),
+        k, v = self._rows(_total(n_tok))
+        check(lib().leap_kv_read_packed(self.handle, layer, n, _iptr(slots),
+                                        _iptr(pos0), _iptr(n_tok), k.data_ptr(),
                                         v.data_ptr()))
         return k, v
 
@@ -199,15 +216,15 @@ class AttentionContext:
         slots = _ints(slots, "slots")
         n = slots.shape[0]
         positions, n_keep = _ints(positions, "positions", n), _ints(n_keep, "n_keep", n)
-        nodes = _ints(nodes, "nodes", int(n_keep.clip(0).sum()))
-        check(lib().leap_kv_keep(self.handle, n, slots.ctypes.data, positions.ctypes.data,
-                                 n_keep.ctypes.data, nodes.ctypes.data))
+        nodes = _ints(nodes, "nodes", _total(n_keep))
+        check(lib().leap_kv_keep(self.handle, n, _iptr(slots), _iptr(positions),
+                                 _iptr(n_keep), _iptr(nodes)))
 
     def _rows(self, n: int):
         import torch
-        shape = (max(n, 0), self.n_kv_heads, self.head_dim)
-        return (torch.empty(shape, dtype=torch.float32, device=f"cuda:{self.device}"),
-                torch.empty(shape, dtype=torch.float32, device=f"cuda:{self.device}"))
+        shape, dev = (max(n, 0), self.n_kv_heads, self.head_dim), torch.device("cuda", self.device)
+        return (torch.empty(shape, dtype=torch.float32, device=dev),
+                torch.empty(shape, dtype=torch.float32, device=dev))
 
     # -- attention ----------------------------------------------------------
     def decode(self, layer: int, pos: int, q, k_new, v_new, out=None):
@@ -239,11 +256,9 @@ class AttentionContext:
             raise ValueError("slots and positions must be equal-length 1-D")
         if out is None:
             out = torch.empty_like(q)
-        ip = ctypes.POINTER(ctypes.c_int)
         check(lib().leap_attn_decode_batched(
-            self.handle, layer, int(slots.shape[0]), slots.ctypes.data_as(ip),
-            positions.ctypes.data_as(ip), _dptr(q), _dptr(k_new), _dptr(v_new),
-            _dptr(out)))
+            self.handle, layer, slots.shape[0], _iptr(slots), _iptr(positions), _dptr(q),
+            _dptr(k_new), _dptr(v_new), _dptr(out)))
         return out
 
     def prefill(self, slot: int, layer: int, pos0: int, q, k, v, out=None):
@@ -259,13 +274,14 @@ class AttentionContext:
         """Device pointers of a ragged call's tensors, their shapes checked."""
         import torch
         qs, ks = (total, self.n_heads, self.head_dim), (total, self.n_kv_heads, self.head_dim)
+        ptrs = [_dptr(q), _dptr(k), _dptr(v)]
         if out is None:
             out = torch.empty_like(q)
-        ptrs = [_dptr(t) for t in (q, k, v, out)]
+        ptrs.append(_dptr(out))
         for name, t, shape in (("q", q, qs), ("k", k, ks), ("v", v, ks), ("out", out, qs)):
-            if tuple(t.shape) != shape:
+            if t.shape != shape:
                 raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
-            if t.device.index != self.device:
+            if t.get_device() != self.device:
                 raise ValueError(f"{name} must be on cuda:{self.device}, got {t.device}")
         return (*ptrs, out)
 
@@ -276,9 +292,9 @@ class AttentionContext:
         slots = _ints(slots, "slots")
         n = slots.shape[0]
         pos0, n_tok = _ints(pos0, "pos0", n), _ints(n_tok, "n_tok", n)
-        qp, kp, vp, op, out = self._packed(int(n_tok.clip(0).sum()), q, k, v, out)
-        check(lib().leap_attn_prefill_packed(self.handle, layer, n, slots.ctypes.data,
-                                             pos0.ctypes.data, n_tok.ctypes.data, qp, kp, vp, op))
+        qp, kp, vp, op, out = self._packed(_total(n_tok), q, k, v, out)
+        check(lib().leap_attn_prefill_packed(self.handle, layer, n, _iptr(slots),
+                                             _iptr(pos0), _iptr(n_tok), qp, kp, vp, op))
         return out
 
     def decode_tree(self, layer: int, slots, positions, n_nodes, parents, q, k, v, out=None):
@@ -291,11 +307,11 @@ class AttentionContext:
         slots = _ints(slots, "slots")
         n = slots.shape[0]
         positions, n_nodes = _ints(positions, "positions", n), _ints(n_nodes, "n_nodes", n)
-        total = int(n_nodes.clip(0).sum())
+        total = _total(n_nodes)
         parents = _ints(parents, "parents", total)
         qp, kp, vp, op, out = self._packed(total, q, k, v, out)
-        check(lib().leap_attn_tree(self.handle, layer, n, slots.ctypes.data, positions.ctypes.data,
-                                   n_nodes.ctypes.data, parents.ctypes.data, qp, kp, vp, op))
+        check(lib().leap_attn_tree(self.handle, layer, n, _iptr(slots), _iptr(positions),
+                                   _iptr(n_nodes), _iptr(parents), qp, kp, vp, op))
         return out
 
     def set_decode_impl(self, impl: int) -> None:

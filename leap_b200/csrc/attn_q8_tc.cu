@@ -675,22 +675,37 @@ q8_tc_join_kernel(const TcArgs a, const __grid_constant__ Q8Seqs tab, const __gr
     if (tok >= tab.tok0[seq + 1] - tok0) return;
     const size_t p0 = size_t(plan.part0[lo] + i * ns) * n_kv + h;  // splits n_kv apart
     const float2 *ml = reinterpret_cast<const float2 *>(a.part_ml) + p0 * kBM + row;
-    const float4 *po = reinterpret_cast<const float4 *>(a.part_o) + (p0 * kBM + row) * (HD / 4) + lane;
-    float mx = -INFINITY;
-    for (int s = lane; s < ns; s += 32) mx = fmaxf(mx, ml[size_t(s) * n_kv * kBM].x);
-#pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-    float sum = 0.f;
+    const float4 *po = reinterpret_cast<const float4 *>(a.part_o) + (p0 * kBM + row) * (HD / 4) + lane % (HD / 4);
+    // 32 splits at a time: lane s has split s's maximum and sum, the row's dims
+    // are spread over the lanes with 8 splits' loads in flight
+    float mx = -INFINITY, sum = 0.f;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int s = 0; s < ns; ++s) {
-        const float2 y = ml[size_t(s) * n_kv * kBM];
-        const float4 z = lane < HD / 4 ? po[size_t(s) * n_kv * kBM * (HD / 4)]
-                                       : make_float4(0.f, 0.f, 0.f, 0.f);
-        if (y.x == -INFINITY) continue;  // the split had nothing this row sees
-        const float e = fast_exp2(y.x - mx);
-        sum += y.y * e;
-        v.x += z.x * e; v.y += z.y * e; v.z += z.z * e; v.w += z.w * e;
+    for (int s0 = 0; s0 < ns; s0 += 32) {
+        const float2 y = s0 + lane < ns ? ml[size_t(s0 + lane) * n_kv * kBM] : make_float2(-INFINITY, 0.f);
+        float top = y.x;
+#pragma unroll
+        for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+        top = fmaxf(top, mx);
+        const float back = mx == -INFINITY ? 0.f : fast_exp2(mx - top);
+        // a split that had nothing this row sees weighs nothing (and was not written)
+        const float e = y.x == -INFINITY ? 0.f : fast_exp2(y.x - top);
+        float part = y.y * e;
+#pragma unroll
+        for (int off = 16; off >= 1; off >>= 1) part += __shfl_xor_sync(0xffffffffu, part, off);
+        mx = top;
+        sum = sum * back + part;
+        v.x *= back; v.y *= back; v.z *= back; v.w *= back;
+        for (int s1 = s0; s1 < min(s0 + 32, ns); s1 += 8) {
+            float4 z[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) z[k] = po[size_t(min(s1 + k, ns - 1)) * n_kv * kBM * (HD / 4)];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float w = __shfl_sync(0xffffffffu, e, s1 + k - s0);
+                if (w == 0.f) continue;
+                v.x += z[k].x * w; v.y += z[k].y * w; v.z += z[k].z * w; v.w += z[k].w * w;
+            }
+        }
     }
     const float inv = 1.f / sum;
     if (lane < HD / 4)
@@ -740,13 +755,13 @@ int launch_tc_g(leap_ctx *c, const TcArgs &a, const Q8Seqs &tab, const Q8TcPlan 
 }
 
 // A block's work apart from its tiles (queries, first loads, output) costs
-// about as much as this many tiles.
-constexpr long kOverhead = 3;
+// about as much as this many tiles, a join of splits as kJoin.
+constexpr long kOverhead = 3, kJoin = 2;
 
 // Sequences longest first, and the tiles of a split.  Blocks are handed to SMs
-// as they fall free, so a launch takes about (all work) / SMs + the longest
-// block; the chunk with the least of that is taken, among those whose partials
-// fit the scratch.
+// as they fall free: one wave takes as long as its longest block, more take about
+// all work / SMs and half the longest block at the end.  The chunk with the least
+// of that is taken, among those whose partials fit the scratch.
 void plan_tc(const leap_ctx *c, const Q8Seqs &tab, bool tree, Q8TcPlan &plan) {
     const int bt = kBM / c->group;
     plan.n = 0;
@@ -763,17 +778,20 @@ void plan_tc(const leap_ctx *c, const Q8Seqs &tab, bool tree, Q8TcPlan &plan) {
     long best = -1;
     plan.chunk = longest;
     for (int chunk = longest; chunk >= 1; chunk = chunk > 16 ? chunk * 7 / 8 : chunk - 1) {
-        long work = 0, parts = 0;
+        long work = 0, parts = 0, items = 0;
         for (int i = 0; i < plan.n; ++i) {
             const int s = plan.seq[i];
             const long tiles = (rows(s) + kBN - 1) / kBN, ns = (tiles + chunk - 1) / chunk;
             // causal tiles see from pos + bt rows on to all of them
             const long mean = tree ? tiles : (tiles + (tab.pos[s] + bt + kBN - 1) / kBN + 1) / 2;
-            work += plan.n_qt[i] * (mean + ns * kOverhead + (ns > 1 ? ns : 0));
+            work += plan.n_qt[i] * (mean + ns * kOverhead);
             if (ns > 1) parts += plan.n_qt[i] * ns;
+            items += plan.n_qt[i] * ns;
         }
         if (parts * c->n_kv > c->q8_tc_parts) break;
-        const long cost = work * c->n_kv / c->num_sms + chunk + kOverhead + (parts ? 2 : 0);
+        const bool wave = items * c->n_kv <= c->num_sms;
+        const long cost = std::max(wave ? 0 : work * c->n_kv / c->num_sms, chunk + kOverhead) +
+                          (wave ? 0 : (chunk + kOverhead) / 2) + (parts ? kJoin : 0);
         if (best < 0 || cost < best) {
             best = cost;
             plan.chunk = chunk;

@@ -151,7 +151,7 @@ int launch_prefill(leap_ctx *c, int slot, int layer, int pos0, int n_tok,
 
 // ---- 8-bit KV cache (kv_q8.cu, attn_q8*.cu) --------------------------------
 constexpr int kMaxTreeNodes = 128;     // nodes of one sequence's tree
-constexpr int kMaxNodesPerLaunch = 4096;
+constexpr int kMaxNodesPerLaunch = 1024;  // (parameters of 2 KB)
 constexpr int kQ8StageRows = 1024;     // rows of k and v that d_rows holds
 
 // A ragged batch of new tokens, by value in kernel parameters: sequence i has
