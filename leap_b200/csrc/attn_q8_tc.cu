@@ -215,6 +215,18 @@ q8_tc_kernel(const __grid_constant__ TcArgs a, const __grid_constant__ Q8Seqs ta
                 load_vec<E / 2>(rc[u], a.rope_cos + c);
                 load_vec<E / 2>(rs[u], a.rope_sin + c);
             }
+            // while they are on their way: what a row sees of the run, itself and its
+            // ancestors (the barrier below makes it known)
+            if (TREE && half == 0) {
+                uint32_t anc[4] = {0u, 0u, 0u, 0u};
+                for (int p = min(t0 + row / G, t_end - 1); p >= 0; p = s_parent[p]) {
+#pragma unroll
+                    for (int w = 0; w < 4; ++w)
+                        if ((p >> 5) == w) anc[w] |= 1u << (p & 31);
+                }
+#pragma unroll
+                for (int w = 0; w < 4; ++w) s_anc[w][row] = anc[w];
+            }
             float fac_of_lane = 0.f;  // lane u: of row u
 #pragma unroll
             for (int u = 0; u < U; ++u) {
@@ -282,17 +294,6 @@ q8_tc_kernel(const __grid_constant__ TcArgs a, const __grid_constant__ Q8Seqs ta
         // those of the run whose bit is set (itself and its ancestors).
         const int tok = t0 + row / G;
         const int lim = pos + min(tok, t_end - 1) + 1;
-        if (TREE && half == 0) {
-            uint32_t anc[4] = {0u, 0u, 0u, 0u};
-            for (int p = min(tok, t_end - 1); p >= 0; p = s_parent[p]) {
-#pragma unroll
-                for (int w = 0; w < 4; ++w)
-                    if ((p >> 5) == w) anc[w] |= 1u << (p & 31);
-            }
-#pragma unroll
-            for (int w = 0; w < 4; ++w) s_anc[w][row] = anc[w];
-        }
-        if (TREE) ok = group_and(ok);
         // bit i: whether key k0 + i is seen
         auto seen = [&](int k0) -> uint32_t {
             if (!TREE) {
@@ -656,7 +657,7 @@ template <int HD, int G>
 __global__ void __launch_bounds__(256)
 q8_tc_join_kernel(const TcArgs a, const __grid_constant__ Q8Seqs tab, const __grid_constant__ Q8TcPlan plan) {
     grid_launch_dependents();
-    grid_dependency_wait();
+    // where things are, while the kernel before runs
     const int lane = threadIdx.x & 31;
     const int n_kv = a.L.n_kv;
     // block: 8 rows of a (query tile, kv head); tiles numbered as in the plan
@@ -668,26 +669,30 @@ q8_tc_join_kernel(const TcArgs a, const __grid_constant__ Q8Seqs tab, const __gr
         if (plan.tile0[mid] <= x) lo = mid; else hi = mid - 1;
     }
     const int ns = plan.nsplit[lo], seq = plan.seq[lo];
-    if (ns == 1) return;
     const int i = x - plan.tile0[lo], qt = plan.n_qt[lo] - 1 - i;
     const int tok = qt * (kBM / G) + row / G;
-    const int tok0 = tab.tok0[seq];
-    if (tok >= tab.tok0[seq + 1] - tok0) return;
+    const int tok0 = tab.tok0[seq], n_new = tab.tok0[seq + 1] - tok0;
     const size_t p0 = size_t(plan.part0[lo] + i * ns) * n_kv + h;  // splits n_kv apart
     const float2 *ml = reinterpret_cast<const float2 *>(a.part_ml) + p0 * kBM + row;
     const float4 *po = reinterpret_cast<const float4 *>(a.part_o) + (p0 * kBM + row) * (HD / 4) + lane % (HD / 4);
+    grid_dependency_wait();
+    if (ns == 1 || tok >= n_new) return;
     // 32 splits at a time: lane s has split s's maximum and sum, the row's dims
-    // are spread over the lanes with 8 splits' loads in flight
+    // are spread over the lanes; 16 splits' loads in flight, the first before the
+    // weights are known
+    constexpr int U = 16;
     float mx = -INFINITY, sum = 0.f;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f), z[U];
     for (int s0 = 0; s0 < ns; s0 += 32) {
         const float2 y = s0 + lane < ns ? ml[size_t(s0 + lane) * n_kv * kBM] : make_float2(-INFINITY, 0.f);
+#pragma unroll
+        for (int k = 0; k < U; ++k) z[k] = po[size_t(min(s0 + k, ns - 1)) * n_kv * kBM * (HD / 4)];
         float top = y.x;
 #pragma unroll
         for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
         top = fmaxf(top, mx);
         const float back = mx == -INFINITY ? 0.f : fast_exp2(mx - top);
-        // a split that had nothing this row sees weighs nothing (and was not written)
+        // a split that had nothing this row sees weighs nothing
         const float e = y.x == -INFINITY ? 0.f : fast_exp2(y.x - top);
         float part = y.y * e;
 #pragma unroll
@@ -695,16 +700,17 @@ q8_tc_join_kernel(const TcArgs a, const __grid_constant__ Q8Seqs tab, const __gr
         mx = top;
         sum = sum * back + part;
         v.x *= back; v.y *= back; v.z *= back; v.w *= back;
-        for (int s1 = s0; s1 < min(s0 + 32, ns); s1 += 8) {
-            float4 z[8];
+        for (int s1 = s0;;) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) z[k] = po[size_t(min(s1 + k, ns - 1)) * n_kv * kBM * (HD / 4)];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const float w = __shfl_sync(0xffffffffu, e, s1 + k - s0);
-                if (w == 0.f) continue;
+            for (int k = 0; k < U; ++k) {
+                const float w = __shfl_sync(0xffffffffu, e, (s1 + k - s0) & 31);
+                if (s1 + k >= ns || w == 0.f) continue;
                 v.x += z[k].x * w; v.y += z[k].y * w; v.z += z[k].z * w; v.w += z[k].w * w;
             }
+            s1 += U;
+            if (s1 >= min(s0 + 32, ns)) break;
+#pragma unroll
+            for (int k = 0; k < U; ++k) z[k] = po[size_t(min(s1 + k, ns - 1)) * n_kv * kBM * (HD / 4)];
         }
     }
     const float inv = 1.f / sum;
