@@ -10,8 +10,7 @@ int q8_attend(leap_ctx *c, int layer, const Q8Seqs &tab, const Q8Tree *tree, con
     for (int i = 0; i < tab.n_seq; ++i)
         if (tab.tok0[i + 1] - tab.tok0[i] > most) most = tab.tok0[i + 1] - tab.tok0[i];
     if (most * c->group <= kQ8Rows) return q8_rows_attend(c, layer, tab, tree, q, k, v, out);
-    if (int st = q8_append(c, layer, tab, tree, k, v)) return st;
-    return q8_tc_attend(c, layer, tab, tree, q, out);
+    return q8_tc_attend(c, layer, tab, tree, q, k, v, out);
 }
 
 }  // namespace leap

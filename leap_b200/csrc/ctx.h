@@ -221,9 +221,8 @@ int q8_rows_parts(const leap_ctx *c);
 int q8_warps_parts(const leap_ctx *c);
 int q8_rows_attend(leap_ctx *c, int layer, const Q8Seqs &tab, const Q8Tree *tree, const float *q,
                    const float *k, const float *v, float *out);
-// The run's rows are stored already.
 int q8_tc_attend(leap_ctx *c, int layer, const Q8Seqs &tab, const Q8Tree *tree, const float *q,
-                 float *out);
+                 const float *k, const float *v, float *out);
 // Append and attend: causal, or a tree of each sequence's tokens.
 int q8_attend(leap_ctx *c, int layer, const Q8Seqs &tab, const Q8Tree *tree, const float *q,
               const float *k, const float *v, float *out);

@@ -230,48 +230,57 @@ int q8_create(leap_ctx *c) {
     c->layer_rows = c->n_kv * c->head_rows;
     c->slot_rows = c->n_layers * c->layer_rows;
     const size_t rows = c->max_batch * c->slot_rows;
-    const size_t stage = 2 * sizeof(float) * kQ8StageRows * c->n_kv * c->hd;
-    cudaError_t e = cudaMalloc(&c->k8, rows * c->hd);
-    if (e == cudaSuccess) e = cudaMalloc(&c->v8, rows * c->hd);
-    if (e == cudaSuccess) e = cudaMalloc(&c->ks8, rows * sizeof(float));
-    if (e == cudaSuccess) e = cudaMalloc(&c->vs8, rows * sizeof(float));
-    if (e == cudaSuccess) e = cudaMalloc(&c->d_rows, stage);
     c->q8_parts = std::max(q8_rows_parts(c), q8_warps_parts(c));
-    const size_t part = size_t(c->q8_parts) * kQ8Rows * sizeof(float);
-    const size_t cnt = size_t(kMaxSeqPerLaunch) * c->n_kv * sizeof(unsigned);
-    if (e == cudaSuccess) e = cudaMalloc(&c->q8_part_o, part * c->hd);
-    if (e == cudaSuccess) e = cudaMalloc(&c->q8_part_ml, part * 2);
-    if (e == cudaSuccess) e = cudaMalloc(&c->q8_counters, cnt);
     c->q8_tc_parts = 4 * c->num_sms;
-    const size_t tc_part = size_t(c->q8_tc_parts) * 128 * sizeof(float);
-    if (e == cudaSuccess) e = cudaMalloc(&c->q8_tc_part_o, tc_part * c->hd);
-    if (e == cudaSuccess) e = cudaMalloc(&c->q8_tc_part_ml, tc_part * 2);
-    if (e == cudaSuccess) e = cudaMemset(c->q8_counters, 0, cnt);
+    // two allocations (each costs a good part of a context's making): the cache, and
+    // everything else; every piece a multiple of 256 bytes
+    const size_t cache = 2 * rows * (c->hd + sizeof(float));
+    char *p = nullptr, *q = nullptr;
+    struct Piece {
+        void **at;
+        size_t bytes;
+    };
+    const size_t f = sizeof(float);
+    const Piece pieces[] = {
+        {reinterpret_cast<void **>(&c->q8_counters), size_t(kMaxSeqPerLaunch) * c->n_kv * sizeof(unsigned)},
+        {reinterpret_cast<void **>(&c->d_rows), 2 * f * kQ8StageRows * c->n_kv * c->hd},
+        {reinterpret_cast<void **>(&c->q8_part_o), f * c->q8_parts * kQ8Rows * c->hd},
+        {reinterpret_cast<void **>(&c->q8_part_ml), f * c->q8_parts * kQ8Rows * 2},
+        {reinterpret_cast<void **>(&c->q8_tc_part_o), f * c->q8_tc_parts * 128 * c->hd},
+        {reinterpret_cast<void **>(&c->q8_tc_part_ml), f * c->q8_tc_parts * 128 * 2},
+    };
+    size_t scratch = 0;
+    for (const Piece &x : pieces) scratch += (x.bytes + 255) / 256 * 256;
+    cudaError_t e = cudaMalloc(&p, cache);
+    if (e == cudaSuccess) {
+        c->k8 = reinterpret_cast<uint8_t *>(p);
+        c->v8 = c->k8 + rows * c->hd;
+        c->ks8 = reinterpret_cast<float *>(c->v8 + rows * c->hd);
+        c->vs8 = c->ks8 + rows;
+        e = cudaMalloc(&q, scratch);
+    }
+    if (e == cudaSuccess) {
+        for (const Piece &x : pieces) {
+            *x.at = q;
+            q += (x.bytes + 255) / 256 * 256;
+        }
+        e = cudaMemset(c->q8_counters, 0, pieces[0].bytes);
+    }
     if (e != cudaSuccess) return cuda_status(e, "cudaMalloc(8-bit cache)");
-    c->device_bytes += 2 * rows * (c->hd + sizeof(float)) + stage + (part + tc_part) * (c->hd + 2) + cnt;
+    c->device_bytes += cache + scratch;
     return q8_clear(c);
 }
 
 void q8_free(leap_ctx *c) {
-    cudaFree(c->k8);
-    cudaFree(c->v8);
-    cudaFree(c->ks8);
-    cudaFree(c->vs8);
-    cudaFree(c->d_rows);
-    cudaFree(c->q8_part_o);
-    cudaFree(c->q8_part_ml);
-    cudaFree(c->q8_counters);
-    cudaFree(c->q8_tc_part_o);
-    cudaFree(c->q8_tc_part_ml);
+    cudaFree(c->k8);           // the cache
+    cudaFree(c->q8_counters);  // the rest
 }
 
 int q8_clear(leap_ctx *c) {
     // code 128 stands for 0; with scale 0 every row reads as zeros
     const size_t rows = c->max_batch * c->slot_rows;
-    cudaError_t e = cudaMemsetAsync(c->k8, 128, rows * c->hd, c->stream);
-    if (e == cudaSuccess) e = cudaMemsetAsync(c->v8, 128, rows * c->hd, c->stream);
-    if (e == cudaSuccess) e = cudaMemsetAsync(c->ks8, 0, rows * sizeof(float), c->stream);
-    if (e == cudaSuccess) e = cudaMemsetAsync(c->vs8, 0, rows * sizeof(float), c->stream);
+    cudaError_t e = cudaMemsetAsync(c->k8, 128, 2 * rows * c->hd, c->stream);  // v8 follows
+    if (e == cudaSuccess) e = cudaMemsetAsync(c->ks8, 0, 2 * rows * sizeof(float), c->stream);
     return cuda_status(e, "clear the 8-bit cache");
 }
 
