@@ -78,18 +78,23 @@ q8_warps_kernel(const __grid_constant__ RowsArgs a, const __grid_constant__ Q8Se
         return s;
     };
     auto first_row = [&](const Segment &s) { return tab.slot[s.seq] * a.L.slot_rows + s.h * a.L.head_rows; };
-    // tile ti of s into the K (0) or V (1) buffer; whole groups of 8 rows (the cache
-    // has room for 128 at a time): rows past the end are read as they are and masked
-    auto ask = [&](const Segment &s, int ti, int v) {
+    // the next tile's first row in the cache, and how many rows of it to copy: whole
+    // groups of 8 (the cache has room for 128 at a time); rows past the end are read
+    // as they are and masked
+    size_t ask_row = 0;
+    int ask_n = 0;
+    auto aim = [&](const Segment &s, int ti) {
+        const int end = tab.pos[s.seq] + tab.tok0[s.seq + 1] - tab.tok0[s.seq];
+        ask_row = first_row(s) + ti * kTile;
+        ask_n = min(kTile, (end - ti * kTile + 7) & ~7);
+    };
+    auto ask = [&](int v) {  // into the K (0) or V (1) buffer
         if (lane == 0) {
-            const size_t row = first_row(s) + ti * kTile;
-            const int end = tab.pos[s.seq] + tab.tok0[s.seq + 1] - tab.tok0[s.seq];
-            const int n = min(kTile, (end - ti * kTile + 7) & ~7);
             unsigned char *st = buf + v * C::kHalf;
             uint64_t *bar = &bars[warp][v];
-            mbar_arrive_expect_tx(bar, n * HD + n * 4);
-            bulk_g2s(st, (v ? a.L.v : a.L.k) + row * HD, n * HD, bar);
-            bulk_g2s(st + kTile * HD, (v ? a.L.vs : a.L.ks) + row, n * 4, bar);
+            mbar_arrive_expect_tx(bar, ask_n * (HD + 4));
+            bulk_g2s(st, (v ? a.L.v : a.L.k) + ask_row * HD, ask_n * HD, bar);
+            bulk_g2s(st + kTile * HD, (v ? a.L.vs : a.L.ks) + ask_row, ask_n * 4, bar);
         }
     };
     // the new rows that fall in tile ti, before it is asked for
@@ -135,9 +140,10 @@ q8_warps_kernel(const __grid_constant__ RowsArgs a, const __grid_constant__ Q8Se
     int ti = at;
     bool on = more;
     const bool early = on && !has_new(sg, ti);
+    if (on) aim(sg, ti);
     if (early) {
-        ask(sg, ti, 0);
-        ask(sg, ti, 1);
+        ask(0);
+        ask(1);
     }
     // Only cached rows of this layer were asked for so far, which the previous
     // kernel of the stream never writes (the host allows the overlap only then).
@@ -145,8 +151,8 @@ q8_warps_kernel(const __grid_constant__ RowsArgs a, const __grid_constant__ Q8Se
     grid_launch_dependents();
     if (on && !early) {
         append(sg, ti);
-        ask(sg, ti, 0);
-        ask(sg, ti, 1);
+        ask(0);
+        ask(1);
     }
 
     uint32_t phase = 0;
@@ -183,8 +189,11 @@ q8_warps_kernel(const __grid_constant__ RowsArgs a, const __grid_constant__ Q8Se
             if (ti + 1 < sg.b) {
                 at = ti + 1;
                 more = true;
+                ask_row += kTile;
+                if (at + 1 == sg.tiles) aim(sg, at);  // the item's last may be short
             } else {
                 settle(sg.next());
+                if (more) aim(as, at);
             }
             const int k0 = ti * kTile, n = pos - k0;  // keys below n are cached
             float s[kTile / 8][2];
@@ -194,7 +203,7 @@ q8_warps_kernel(const __grid_constant__ RowsArgs a, const __grid_constant__ Q8Se
             __syncwarp();
             if (more) {
                 if (has_new(as, at)) append(as, at);
-                ask(as, at, 0);
+                ask(0);
             }
             if (n < kTile) {
                 const int mine = g / G;  // token of row g
@@ -211,7 +220,7 @@ q8_warps_kernel(const __grid_constant__ RowsArgs a, const __grid_constant__ Q8Se
             const float *svs = reinterpret_cast<const float *>(buf + C::kHalf + kTile * HD);
             M::absorb(buf + C::kHalf, svs, top_scale(lane < n + n_new ? svs[lane] : 0.f), s, m, l, o);
             __syncwarp();
-            if (more) ask(as, at, 1);
+            if (more) ask(1);
             phase ^= 1;
             if (ti + 1 >= sg.b) break;
         }

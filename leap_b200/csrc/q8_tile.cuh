@@ -47,6 +47,16 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// The same from zero.
+__device__ __forceinline__ void mma_f16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                              uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
 // Two of four bytes x (codes + 128) as FP16 values code, code.
 template <int SEL>
 __device__ __forceinline__ uint32_t half_pair(uint32_t x) {
@@ -67,8 +77,6 @@ struct TileMath {
         const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
         float cc[NK / 8][4];
 #pragma unroll
-        for (int n = 0; n < NK / 8; ++n) cc[n][0] = cc[n][1] = cc[n][2] = cc[n][3] = 0.f;
-#pragma unroll
         for (int j = 0; j < HD / 64; ++j) {
             // this thread's 16 dims of the query's rows: 4 steps
             const uint4 *h = reinterpret_cast<const uint4 *>(sq + g * HD + 16 * (t + 4 * j));
@@ -81,9 +89,11 @@ struct TileMath {
                 const uint4 w = *reinterpret_cast<const uint4 *>(sk + q8_chunk<HD>(n * 8 + g, t + 4 * j));
                 const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-                for (int u = 0; u < 4; ++u)
-                    mma_f16(cc[n], qh[2 * u], ql[2 * u], qh[2 * u + 1], ql[2 * u + 1], half_pair<0x5140>(ww[u]),
-                            half_pair<0x5342>(ww[u]));
+                for (int u = 0; u < 4; ++u) {
+                    const uint32_t b0 = half_pair<0x5140>(ww[u]), b1 = half_pair<0x5342>(ww[u]);
+                    if (j + u == 0) mma_f16_first(cc[n], qh[0], ql[0], qh[1], ql[1], b0, b1);
+                    else mma_f16(cc[n], qh[2 * u], ql[2 * u], qh[2 * u + 1], ql[2 * u + 1], b0, b1);
+                }
             }
         }
 #pragma unroll
@@ -133,8 +143,6 @@ struct TileMath {
         for (int part = 0; part < PARTS; ++part) {
             float acc[NT / PARTS][4];
 #pragma unroll
-            for (int i = 0; i < NT / PARTS; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
-#pragma unroll
             for (int kk = 0; kk < NK / 16; ++kk) {
                 constexpr int NW = HD / 32 / PARTS;  // words of a row
                 uint32_t w[4][NW];
@@ -158,10 +166,14 @@ struct TileMath {
                 for (int j = 0; j < NW; ++j) {
                     const uint32_t ab0 = __byte_perm(w[0][j], w[1][j], 0x5140), ab1 = __byte_perm(w[0][j], w[1][j], 0x7362);
                     const uint32_t cd0 = __byte_perm(w[2][j], w[3][j], 0x5140), cd1 = __byte_perm(w[2][j], w[3][j], 0x7362);
-                    mma_f16(acc[4 * j + 0], a0, a1, a2, a3, half_pair<0x5140>(ab0), half_pair<0x5140>(cd0));
-                    mma_f16(acc[4 * j + 1], a0, a1, a2, a3, half_pair<0x5342>(ab0), half_pair<0x5342>(cd0));
-                    mma_f16(acc[4 * j + 2], a0, a1, a2, a3, half_pair<0x5140>(ab1), half_pair<0x5140>(cd1));
-                    mma_f16(acc[4 * j + 3], a0, a1, a2, a3, half_pair<0x5342>(ab1), half_pair<0x5342>(cd1));
+                    auto mma = [&](float (&d)[4], uint32_t b0, uint32_t b1) {
+                        if (kk == 0) mma_f16_first(d, a0, a1, a2, a3, b0, b1);
+                        else mma_f16(d, a0, a1, a2, a3, b0, b1);
+                    };
+                    mma(acc[4 * j + 0], half_pair<0x5140>(ab0), half_pair<0x5140>(cd0));
+                    mma(acc[4 * j + 1], half_pair<0x5342>(ab0), half_pair<0x5342>(cd0));
+                    mma(acc[4 * j + 2], half_pair<0x5140>(ab1), half_pair<0x5140>(cd1));
+                    mma(acc[4 * j + 3], half_pair<0x5342>(ab1), half_pair<0x5342>(cd1));
                 }
             }
 #pragma unroll
