@@ -669,6 +669,105 @@ def test_rows_past_four_gigabytes(cuda):
         np.testing.assert_array_equal(ctx.kv_read(63, 0, 70013, 3)[0], stored(x))
 
 
+# ---- batches that the kernel of single warps takes ---------------------------------------
+@pytest.mark.parametrize("shape", ["l8b", "l70b", "g8_64"])
+def test_decode_of_many_sequences(cuda, shape):
+    """More (sequence, kv head) pairs than blocks run at once, two steps."""
+    rng = np.random.default_rng(31)
+    n = 320 // ALL[shape][1]
+    with make(shape, 1100, max_batch=n, n_layers=2) as ctx:
+        rows = rng.integers(0, 1000, n)
+        rows[:6] = [0, 1, 31, 32, 33, 64]
+        r = Ragged(ctx, rng, rng.permutation(n), rows, layer=1)
+        for _ in range(2):
+            q, k, v = r.inputs([1] * n)
+            r.check(ctx.decode_batched(1, r.slots, r.rows, *gpu(q, k, v)), q, k, v, [1] * n)
+        kk, vv = ctx.kv_read(0, 0, 0, 1100)
+        assert not kk.any() and not vv.any()
+
+
+def test_decode_of_items_in_many_parts(cuda):
+    """Long contexts: every item is spread over many warps and joined."""
+    rng = np.random.default_rng(32)
+    with make("l8b", 6200, max_batch=16) as ctx:
+        r = Ragged(ctx, rng, rng.permutation(16), rng.integers(5500, 6100, 16))
+        q, k, v = r.inputs([1] * 16)
+        out = ctx.decode_batched(0, r.slots, r.rows, *gpu(q, k, v)).cpu().numpy()
+        for i in (0, 7, 15):
+            ref, kn, vn = attend(ctx, r.k[i], r.v[i], q[i:i + 1], k[i:i + 1], v[i:i + 1])
+            near(out[i:i + 1], ref)
+            kk, vv = ctx.kv_read(int(r.slots[i]), 0, int(r.rows[i]), 1)
+            np.testing.assert_array_equal(kk, kn)
+            np.testing.assert_array_equal(vv, vn)
+
+
+@pytest.mark.parametrize("shape,most", [("mha128", 8), ("g2_64", 4), ("l8b", 2), ("l70b", 1)])
+def test_small_trees_of_many_sequences(cuda, shape, most):
+    """New rows that straddle tiles of 32 rows, sequences without any, NaN behind."""
+    rng = np.random.default_rng(33)
+    n = 60
+    lens = [int(x) for x in rng.integers(0, most + 1, n)]
+    lens[0] = most
+    rows = 32 * rng.integers(0, 12, n) + rng.integers(24, 34, n)
+    with make(shape, 500, max_batch=n) as ctx:
+        r = Ragged(ctx, rng, rng.permutation(n), rows)
+        for s, c in zip(r.slots, rows):
+            poison(ctx, int(s), int(c), 500)
+        q, k, v = r.inputs(lens)
+        par = np.concatenate([tree(rng, t) for t in lens])
+        r.check(ctx.decode_tree(0, r.slots, r.rows, lens, par, *gpu(q, k, v)), q, k, v, lens, par)
+        q, k, v = r.inputs(lens)
+        r.check(ctx.prefill_packed(0, r.slots, r.rows, lens, *gpu(q, k, v)), q, k, v, lens)
+
+
+@pytest.mark.parametrize("shape", ["l8b", "tl", "mha128"])
+@pytest.mark.parametrize("pos", [127, 250, 1020, 2040, 4090])
+def test_new_rows_across_tiles_and_splits(cuda, shape, pos):
+    """One query tile a sequence: its blocks store the new rows themselves, each
+    those of its own range."""
+    rng = np.random.default_rng(34)
+    with make(shape, pos + 40) as ctx:
+        r = Ragged(ctx, rng, [0], [pos])
+        for n in (16, 11):
+            q, k, v = r.inputs([n])
+            par = tree(rng, n)
+            r.check(ctx.decode_tree(0, [0], r.rows, [n], par, *gpu(q, k, v)), q, k, v, [n], par)
+
+
+def test_layers_back_to_back_of_every_kind(cuda):
+    """Decode, trees and prompts on layers in turn without a wait between them give
+    what they give with one."""
+    rng = np.random.default_rng(35)
+    h, kv, hd = ALL["l8b"]
+    ops = [("d", 0, 1), ("t", 1, 9), ("d", 0, 1), ("p", 2, 70), ("d", 1, 1), ("t", 0, 2), ("d", 2, 1), ("t", 2, 60),
+           ("d", 0, 1), ("d", 2, 1), ("p", 0, 3), ("d", 1, 1)]
+    ins = [gpu(rnd(rng, n, h, hd), rnd(rng, n, kv, hd), rnd(rng, n, kv, hd)) for _, _, n in ops]
+    par = [tree(rng, n) for _, _, n in ops]
+    base = [(rnd(rng, 1500, kv, hd), rnd(rng, 1500, kv, hd)) for _ in range(3)]
+    got = []
+    for wait in (True, False):
+        with make("l8b", 1800, n_layers=3) as ctx:
+            for layer, (k, v) in enumerate(base):
+                ctx.kv_write(0, layer, 0, k, v)
+            pos, outs = [1500] * 3, []
+            for (what, layer, n), x, p in zip(ops, ins, par):
+                if what == "d":
+                    outs.append(ctx.decode_batched(layer, [0], [pos[layer]], *x))
+                elif what == "t":
+                    outs.append(ctx.decode_tree(layer, [0], [pos[layer]], [n], p, *x))
+                else:
+                    outs.append(ctx.prefill_packed(layer, [0], [pos[layer]], [n], *x))
+                pos[layer] += n
+                if wait:
+                    ctx.sync()
+            ctx.sync()
+            got.append((torch.cat(outs).cpu(), [ctx.kv_read(0, i, 1500, 300) for i in range(3)]))
+    assert torch.equal(got[0][0], got[1][0])
+    for a, b in zip(got[0][1], got[1][1]):
+        np.testing.assert_array_equal(a[0], b[0])
+        np.testing.assert_array_equal(a[1], b[1])
+
+
 # ---- the engine ---------------------------------------------------------------------------
 @pytest.mark.parametrize("quantized", [False, True])
 def test_engine_with_an_8_bit_cache(cuda, quantized):
