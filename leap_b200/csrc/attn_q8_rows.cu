@@ -11,8 +11,8 @@
 // than the bytes, so the products run on mma.sync (q8_tile.cuh).  tcgen05 has
 // nothing to give here: its 128-row tiles would be 16 times empty.
 //
-// This kernel is for little work (see q8_rows_attend): splits of one wave, a block
-// each.
+// This kernel is for little work (see q8_rows_attend): splits of a sequence, a block
+// each, in one wave where that is best.
 //  * A warp works alone: it streams its own tiles of 32 rows (K and V codes and
 //    scales, one bulk copy each) through its own ring of shared-memory buffers
 //    and keeps its own running maximum, sum and output.  No barrier is shared
@@ -333,41 +333,55 @@ int launch_rows_g(leap_ctx *c, const RowsArgs &a, const Q8Seqs &tab, const Q8Spl
                 : launch_rows<HD, G, false>(c, a, tab, plan, Q8See<false>(), overlap);
 }
 
-// Rows of a split: one wave of one block an SM, at least kMinChunk (a partial
-// costs as much as some rows).
+// Rows of a split, at least kMinChunk.  What a batch costs, in rows that a block
+// streams (140 a us with 128 dims, 220 with 64): a block besides its rows kBlock, the
+// joins at the end kJoin (8 kv heads of 128 on the device, sequences x cached rows:
+// 1x128, one block each, 5.4 us; 1x512 in 4 splits 8.2; 16x8192, one each, 61;
+// 32x2048, two waves, 40).
 constexpr int kMinChunk = 128;
+constexpr long kBlock = 512, kJoin = 320;
 
-void plan_splits(const leap_ctx *c, const Q8Seqs &tab, Q8Splits &plan) {
+// Splits with the least cost; returns it.  One wave of a block an SM takes as long as
+// its longest, more take about all work / SMs and half the longest block at the end.
+long plan_splits(const leap_ctx *c, const Q8Seqs &tab, Q8Splits &plan) {
     long total = 0;
+    unsigned longest = 0, n_any = 0;
     for (int i = 0; i < tab.n_seq; ++i)
-        if (tab.tok0[i + 1] > tab.tok0[i]) total += tab.pos[i];
-    long chunk = (total * c->n_kv + c->num_sms - 1) / c->num_sms;
-    chunk = std::max((chunk + 63) / 64 * 64, long(kMinChunk));
-    auto splits = [&](int i, long ch) {
-        return tab.tok0[i + 1] == tab.tok0[i] ? 0 : std::max((tab.pos[i] + ch - 1) / ch, 1L);
-    };
-    // one wave, if the sequences' last splits do not push past it
-    for (;; chunk += 64) {
-        long n = 0, most = 0;
-        for (int i = 0; i < tab.n_seq; ++i) {
-            n += splits(i, chunk);
-            most = std::max(most, splits(i, chunk));
+        if (tab.tok0[i + 1] > tab.tok0[i]) {
+            total += tab.pos[i];
+            longest = std::max(longest, unsigned(tab.pos[i]));
+            ++n_any;
         }
-        if (n * c->n_kv <= c->num_sms || most <= 1) break;
+    auto splits = [&](int i, unsigned ch) {
+        return tab.tok0[i + 1] == tab.tok0[i] ? 0u : std::max((unsigned(tab.pos[i]) + ch - 1) / ch, 1u);
+    };
+    long best = -1;
+    unsigned ch = unsigned(std::max(((total * c->n_kv + c->num_sms - 1) / c->num_sms + 63) / 64 * 64, long(kMinChunk)));
+    // finer steps where one wave can be had
+    const int step = long(n_any) * c->n_kv <= c->num_sms ? 16 : 2;
+    for (;; ch += std::max(ch / step / 64 * 64, 64u)) {
+        long n = 0;
+        for (int i = 0; i < tab.n_seq; ++i) n += splits(i, ch);
+        const bool split = longest > ch, wave = n * c->n_kv <= c->num_sms;
+        const long last = std::min(ch, longest) + kBlock;
+        const long cost = (wave ? last : std::max((total + n * kBlock) * c->n_kv / c->num_sms, last) + last / 2) +
+                          (split ? kJoin : 0);
+        if ((!split || n * c->n_kv <= c->q8_parts) && (best < 0 || cost < best)) {
+            best = cost;
+            plan.chunk = int(ch);
+        }
+        if (wave || !split) break;
     }
-    plan.chunk = int(chunk);
     int n = 0;
     for (int i = 0; i < tab.n_seq; ++i) {
         plan.split0[i] = n;
-        n += int(splits(i, chunk));
+        n += int(splits(i, unsigned(plan.chunk)));
     }
     plan.split0[tab.n_seq] = n;
+    return best;
 }
 
 }  // namespace
-
-// Splits (if any sequence has more than one) fit one wave.
-int q8_rows_parts(const leap_ctx *c) { return c->num_sms; }
 
 int q8_rows_attend(leap_ctx *c, int layer, const Q8Seqs &tab, const Q8Tree *tree, const float *q,
                    const float *k, const float *v, float *out) {
@@ -388,9 +402,14 @@ int q8_rows_attend(leap_ctx *c, int layer, const Q8Seqs &tab, const Q8Tree *tree
     // as launch_decode: only if the previous operation did not write this layer
     const bool overlap = c->overlap && c->last_written_layer != leap_ctx::kWroteAll &&
                          c->last_written_layer != layer;
-    if (q8_warps_fit(c, tab)) return q8_warps_launch(c, a, tab, tree, overlap);
     Q8Splits plan;
-    plan_splits(c, tab, plan);
+    // Measured against expected (device us of the rows, warps kernel; 8 kv heads of 128,
+    // 4 query heads each): 1x8192 10.1, 44.8; 8x8192 35.4, 41.0; 16x8192 60.6, 58.5;
+    // 20x2048 35.6, 26.5; 64x512 33.2, 23.6; 64x8192 239, 180; one of 32768 among 20
+    // short ones 34, 90, among 64 65, 68; 4x32768 63, 73; 8x32768 118, 105.  Of 222
+    // batches (heads 32/8, 32/32, 16/2 and 8/1 of 128, 32/8 and 32/4 of 64) the taken one
+    // was within 10% of the other in all but one (36x1024 of 32/8x64: 18.5, 15.2).
+    if (q8_warps_cost(c, tab) < plan_splits(c, tab, plan)) return q8_warps_launch(c, a, tab, tree, overlap);
     switch (c->hd * 100 + c->group) {
         case 12801: return launch_rows_g<128, 1>(c, a, tab, plan, tree, overlap);
         case 12802: return launch_rows_g<128, 2>(c, a, tab, plan, tree, overlap);

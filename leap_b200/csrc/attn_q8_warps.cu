@@ -9,7 +9,7 @@
 // an item ends it stages the next item's queries and leaves its part of the sums,
 // or the output, alone: no block ever waits for its warps, so the other 15 of an
 // SM keep the copies going.  64 sequences of 512 to 8192 rows, 8 kv heads of 128:
-// 107 us, 5.3 TB/s; blocks that walked such a list together lost about 9 us an item
+// 105 us, 5.45 TB/s; blocks that walked such a list together lost about 9 us an item
 // to their joins (141 us).  The parts of an item are joined by the warp that is last (atomic
 // ticket).  The products are those of q8_tile.cuh.
 //
@@ -353,19 +353,16 @@ void plan_units(const leap_ctx *c, const Q8Seqs &tab, Q8Units &plan, int *longes
 // Two partials a warp.
 int q8_warps_parts(const leap_ctx *c) { return 2 * 2 * kWarps * c->num_sms; }
 
-// Which batches.  The rows kernel's blocks join their warps and so finish a short
-// list sooner; this kernel keeps more copies in flight.  Device us of (this, rows)
-// kernel at 8 kv heads of 128, 4 query heads each, seqs x cached rows: 1x8192 46,
-// 11.7; 8x8192 44, 39; 32x512 19.5, 17.3; 16x8192 62, 64; 32x2048 42, 44; 64x128
-// 15, 20; 64x512 24, 33; 64x8192 191, 245; 4x32768 77, 66 (one warp joins 74 parts);
-// 8x32768 111, 121 (37 parts).  So: 8 tiles a warp, or more items than the rows
-// kernel has blocks at once; and an item in at most 40 parts.
-bool q8_warps_fit(const leap_ctx *c, const Q8Seqs &tab) {
+// What a batch costs here, in the unit of the rows kernel's plan (1/140 us with 128
+// dims): a warp's tiles, and one warp's join of the item in most parts, 8 of a row at a
+// time (1x8192 of 8 kv heads, 129 parts: 45 us with 4 rows, 80 with 8).
+long q8_warps_cost(const leap_ctx *c, const Q8Seqs &tab) {
     Q8Units plan;
-    int longest, items = 0;
+    int longest;
     plan_units(c, tab, plan, &longest);
-    for (int i = 0; i < tab.n_seq; ++i) items += tab.tok0[i + 1] > tab.tok0[i] ? c->n_kv : 0;
-    return (plan.chunk >= 8 || items > 2 * c->num_sms) && (longest + plan.chunk - 1) / plan.chunk <= 40;
+    int rows = 0;
+    for (int i = 0; i < tab.n_seq; ++i) rows = std::max(rows, (tab.tok0[i + 1] - tab.tok0[i]) * c->group);
+    return 1080 + 450L * plan.chunk + 9L * rows * ((longest + plan.chunk - 1) / plan.chunk);
 }
 
 int q8_warps_launch(leap_ctx *c, const RowsArgs &a, const Q8Seqs &tab, const Q8Tree *tree, bool overlap) {

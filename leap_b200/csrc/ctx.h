@@ -217,7 +217,6 @@ int q8_append(leap_ctx *c, int layer, const Q8Seqs &tab, const Q8Tree *tree, con
 int kv_read_packed(leap_ctx *c, int layer, const Q8Seqs &tab, float *k, float *v);
 // Move rows pos + at[j] to pos + j (j counted from each sequence's first).
 int kv_keep(leap_ctx *c, const Q8Seqs &tab, const Q8Nodes &nodes);
-int q8_rows_parts(const leap_ctx *c);
 int q8_warps_parts(const leap_ctx *c);
 int q8_rows_attend(leap_ctx *c, int layer, const Q8Seqs &tab, const Q8Tree *tree, const float *q,
                    const float *k, const float *v, float *out);

@@ -230,7 +230,7 @@ int q8_create(leap_ctx *c) {
     c->layer_rows = c->n_kv * c->head_rows;
     c->slot_rows = c->n_layers * c->layer_rows;
     const size_t rows = c->max_batch * c->slot_rows;
-    c->q8_parts = std::max(q8_rows_parts(c), q8_warps_parts(c));
+    c->q8_parts = q8_warps_parts(c);  // the rows kernel keeps to as many
     c->q8_tc_parts = 4 * c->num_sms;
     // two allocations (each costs a good part of a context's making): the cache, and
     // everything else; every piece a multiple of 256 bytes

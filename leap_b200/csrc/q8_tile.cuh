@@ -34,8 +34,8 @@ struct RowsArgs {
     float scale_log2;
 };
 
-// attn_q8_warps.cu: whether a batch is for it, and its launch.
-bool q8_warps_fit(const leap_ctx *c, const Q8Seqs &tab);
+// attn_q8_warps.cu: what a batch costs there, and its launch.
+long q8_warps_cost(const leap_ctx *c, const Q8Seqs &tab);
 int q8_warps_launch(leap_ctx *c, const RowsArgs &a, const Q8Seqs &tab, const Q8Tree *tree, bool overlap);
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,

@@ -701,6 +701,24 @@ def test_decode_of_items_in_many_parts(cuda):
             np.testing.assert_array_equal(vv, vn)
 
 
+@pytest.mark.parametrize("shape,nodes", [("l8b", 1), ("l8b", 2), ("g2_64", 1), ("l70b", 1)])
+def test_one_long_sequence_among_short_ones(cuda, shape, nodes):
+    """Splits of the long one, more blocks than run at once; it comes last."""
+    rng = np.random.default_rng(37)
+    n = 160 // ALL[shape][1] + 3
+    with make(shape, 6000, max_batch=n) as ctx:
+        rows = rng.integers(0, 130, n)
+        rows[:3] = [0, 127, 128]
+        rows[-1] = 5990
+        r = Ragged(ctx, rng, rng.permutation(n), rows)
+        q, k, v = r.inputs([nodes] * n)
+        if nodes == 1:
+            out = ctx.decode_batched(0, r.slots, r.rows, *gpu(q, k, v))
+        else:
+            out = ctx.prefill_packed(0, r.slots, r.rows, [nodes] * n, *gpu(q, k, v))
+        r.check(out, q, k, v, [nodes] * n)
+
+
 @pytest.mark.parametrize("shape,most", [("mha128", 8), ("g2_64", 4), ("l8b", 2), ("l70b", 1)])
 def test_small_trees_of_many_sequences(cuda, shape, most):
     """New rows that straddle tiles of 32 rows, sequences without any, NaN behind."""
