@@ -25,7 +25,8 @@
 //   warps 8-11       codes -> FP16 operand tiles (128-byte swizzle; V is used
 //                    N-major, so nothing is transposed), a tile ahead in
 //                    registers, and the tile's scales.
-//   warps 13-15      store the block's new rows, where that is left to it.
+//   warps 13-15      store the block's new rows, where that is left to it (with the
+//                    softmax warps' help, where its first tiles have them).
 //   warp 12          issues the products: S(j+1) = Q K^T, then O(j) = P V.
 // TMEM: two buffers of S/P (128 columns each), O (HD) and Q hi/lo (HD): both
 // products take their A operand from TMEM, since two operands in shared memory
@@ -77,7 +78,7 @@ struct TcArgs {
 
 struct TcBars {
     uint64_t q_ready;    // Q in TMEM (8 softmax warps)
-    uint64_t new_full;   // the block's new rows are stored (warps 13-15)
+    uint64_t new_full;   // the block's new rows are stored (n_app warps)
     uint64_t k_full[2], v_full[2];  // operand tile in place (4 converter warps)
     uint64_t sc_full[kSlots];       // scales of a tile in place (4 converter warps)
     uint64_t s_full[2];  // S(j) done: K buffer free (commit)
@@ -173,9 +174,14 @@ q8_tc_kernel(const __grid_constant__ TcArgs a, const __grid_constant__ Q8Seqs ta
     const int j0 = it.split * plan.chunk;
     const int n_kt = max(min(n_all - j0, plan.chunk), 0);  // tiles j0 .. j0 + n_kt - 1
 
+    // The run's rows that this block reads, where it stores them: i0 .. i1 - 1.  Warps
+    // 13-15 do it beside the first tiles; where these need the rows, the softmax warps help.
+    const int i0 = max(j0 * kBN - pos, 0), i1 = a.k_new ? max(min((j0 + n_kt) * kBN - pos, n_new), i0) : i0;
+    const int n_app = i1 - i0 > 6 * (max(pos - j0 * kBN, 0) / kBN) ? 11 : 3;
+
     if (tid == 0) {
         mbar_init(&bars.q_ready, 8);
-        mbar_init(&bars.new_full, 3);
+        mbar_init(&bars.new_full, n_app);
         for (int b = 0; b < 2; ++b) {
             mbar_init(&bars.k_full[b], 4);
             mbar_init(&bars.v_full[b], 4);
@@ -197,6 +203,30 @@ q8_tc_kernel(const __grid_constant__ TcArgs a, const __grid_constant__ Q8Seqs ta
     __syncthreads();
     tc::fence_after_sync();
     const uint32_t tmem = tmem_sh;
+    // Warp w's part of the new rows, U of them (k or v) in flight at a time.
+    auto append = [&](auto u_, int w) {
+        constexpr int U = decltype(u_)::value;
+        const size_t r0 = tab.slot[seq] * a.L.slot_rows + h * a.L.head_rows;
+        for (int x = 2 * i0 + w; x < 2 * i1; x += U * n_app) {
+            Q8NewRow<HD> r[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int y = x + u * n_app, i = y >> 1;
+                if (y < 2 * i1)
+                    r[u].load((y & 1 ? a.v_new : a.k_new) + (size_t(tok0 + i) * a.L.n_kv + h) * HD, !(y & 1), a.rope_cos,
+                              a.rope_sin, pos + see.depth(tok0, i));
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int y = x + u * n_app;
+                uint32_t codes;
+                if (y < 2 * i1)
+                    r[u].store(!(y & 1), (y & 1 ? a.L.v : a.L.k) + r0 * HD, (y & 1 ? a.L.vs : a.L.ks) + r0, pos + (y >> 1), codes);
+            }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.new_full);
+    };
 
     if (warp < 8) {
         // ================= softmax groups =====================================
@@ -294,6 +324,7 @@ q8_tc_kernel(const __grid_constant__ TcArgs a, const __grid_constant__ Q8Seqs ta
         tc::fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars.q_ready);
+        if (n_app > 3) append(std::integral_constant<int, 4>(), 3 + warp);
 
         // What this row sees: keys below `lim`, or (TREE) keys below pos and
         // those of the run whose bit is set (itself and its ancestors).
@@ -593,18 +624,7 @@ q8_tc_kernel(const __grid_constant__ TcArgs a, const __grid_constant__ Q8Seqs ta
         regs_down<kRegsIssue>();
         if (warp > 12 && a.k_new) {
             // ================= the run's rows that this block reads =============
-            const size_t r0 = tab.slot[seq] * a.L.slot_rows + h * a.L.head_rows;
-            const int i0 = max(j0 * kBN - pos, 0), i1 = min((j0 + n_kt) * kBN - pos, n_new);
-            for (int x = 2 * i0 + warp - 13; x < 2 * i1; x += 3) {
-                const int i = x >> 1;
-                const bool is_v = x & 1;
-                uint32_t codes;
-                q8_append_row<HD>((is_v ? a.v_new : a.k_new) + (size_t(tok0 + i) * a.L.n_kv + h) * HD, !is_v,
-                                  a.rope_cos, a.rope_sin, pos + see.depth(tok0, i), (is_v ? a.L.v : a.L.k) + r0 * HD,
-                                  (is_v ? a.L.vs : a.L.ks) + r0, pos + i, codes);
-            }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bars.new_full);
+            append(std::integral_constant<int, 1>(), warp - 13);
         }
         if (warp == 12) {
             // ================= MMA issuer ======================================
@@ -859,10 +879,14 @@ int q8_tc_attend(leap_ctx *c, int layer, const Q8Seqs &tab, const Q8Tree *tree, 
     Q8TcPlan plan;
     plan_tc(c, tab, tree != nullptr, plan);
     // One query tile a sequence: every new row is read by one block, which can store
-    // it itself (a launch less: 5 nodes on 300 rows, 13.2 -> 12.1 us on the device and
-    // 4 us less to issue).  Otherwise several blocks read it.
+    // it itself (a launch less: 5 nodes on 300 rows, 13.2 -> 11.6 us on the device and
+    // 4 us less to issue), unless there are many (32 kv heads, device us of appended
+    // by the blocks and by the kernel: 16 rows 11.8, 10.9; 64 rows 15.7, 11.9; 128 rows
+    // 20.8, 13.0; 4 x 64 behind 2000 43.9, 46.1).  Otherwise several blocks read it.
+    constexpr int kMostFused = 64;
     bool fused = true;
-    for (int i = 0; i < plan.n; ++i) fused = fused && plan.n_qt[i] == 1;
+    for (int i = 0; i < plan.n; ++i)
+        fused = fused && plan.n_qt[i] == 1 && tab.tok0[plan.seq[i] + 1] - tab.tok0[plan.seq[i]] <= kMostFused;
     if (!fused)
         if (int st = q8_append(c, layer, tab, tree, k, v)) return st;
     TcArgs a;

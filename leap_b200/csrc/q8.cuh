@@ -154,31 +154,45 @@ __device__ __forceinline__ uint32_t q8_load_codes(const uint8_t *head, int r, in
     return *reinterpret_cast<const uint16_t *>(head + q8_chunk<HD>(r, lane >> 3) + (lane & 7) * 2);
 }
 
-// A warp rotates (k) and quantises a new row and stores it as row `row` of its
-// head; `codes` and the scale (every lane's) come back.
+// A new row as a warp takes it: the lane's dims, and for k what rotates them.
+template <int HD>
+struct Q8NewRow {
+    static constexpr int E = HD / 32;
+    float x[E], rc[E / 2], rs[E / 2];
+
+    __device__ __forceinline__ void load(const float *src, bool is_k, const float *rope_cos, const float *rope_sin, int at) {
+        const int lane = threadIdx.x & 31;
+        load_vec<E>(x, src + E * lane);
+        if (is_k) {
+            const size_t c = size_t(at) * (HD / 2) + lane * (E / 2);
+            load_vec<E / 2>(rc, rope_cos + c);
+            load_vec<E / 2>(rs, rope_sin + c);
+        }
+    }
+    // Rotates (k), quantises and stores it as row `row` of its head; `codes` and the
+    // scale (every lane's) come back.
+    __device__ __forceinline__ float store(bool is_k, uint8_t *head, float *scales, int row, uint32_t &codes) {
+        const int lane = threadIdx.x & 31;
+        if (is_k) {
+#pragma unroll
+            for (int e = 0; e < E; e += 2) {
+                const float2 z = rope_pair(x[e], x[e + 1], rc[e / 2], rs[e / 2]);
+                x[e] = z.x;
+                x[e + 1] = z.y;
+            }
+        }
+        const float s = q8_quantize<E>(x, codes);
+        q8_store_codes<HD>(head, row, lane, codes);
+        if (lane == 0) scales[row] = s;
+        return s;
+    }
+};
 template <int HD>
 __device__ __forceinline__ float q8_append_row(const float *src, bool is_k, const float *rope_cos, const float *rope_sin,
                                                int at, uint8_t *head, float *scales, int row, uint32_t &codes) {
-    constexpr int E = HD / 32;
-    const int lane = threadIdx.x & 31;
-    float x[E];
-    load_vec<E>(x, src + E * lane);
-    if (is_k) {
-        float rc[E / 2], rs[E / 2];
-        const size_t c = size_t(at) * (HD / 2) + lane * (E / 2);
-        load_vec<E / 2>(rc, rope_cos + c);
-        load_vec<E / 2>(rs, rope_sin + c);
-#pragma unroll
-        for (int e = 0; e < E; e += 2) {
-            const float2 z = rope_pair(x[e], x[e + 1], rc[e / 2], rs[e / 2]);
-            x[e] = z.x;
-            x[e + 1] = z.y;
-        }
-    }
-    const float s = q8_quantize<E>(x, codes);
-    q8_store_codes<HD>(head, row, lane, codes);
-    if (lane == 0) scales[row] = s;
-    return s;
+    Q8NewRow<HD> r;
+    r.load(src, is_k, rope_cos, rope_sin, at);
+    return r.store(is_k, head, scales, row, codes);
 }
 
 }  // namespace leap

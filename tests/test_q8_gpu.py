@@ -701,6 +701,23 @@ def test_decode_of_items_in_many_parts(cuda):
             np.testing.assert_array_equal(vv, vn)
 
 
+@pytest.mark.parametrize("shape", ["mha128", "mha64", "g2_64"])
+@pytest.mark.parametrize("drafted", [False, True])
+def test_new_rows_that_few_or_many_warps_store(cuda, shape, drafted):
+    """Up to a query tile of new rows, in a block's first tiles and further on."""
+    rng = np.random.default_rng(38)
+    for lens in ([9, 64, 13], [17, 64, 50], [128 if shape != "g2_64" else 64, 65, 3]):
+        with make(shape, 1500, max_batch=3) as ctx:
+            r = Ragged(ctx, rng, [2, 0, 1], [0, 125, 1300])
+            q, k, v = r.inputs(lens)
+            if drafted:
+                parents = np.concatenate([tree(rng, n) for n in lens])
+                out = ctx.decode_tree(0, r.slots, r.rows, lens, parents, *gpu(q, k, v))
+                r.check(out, q, k, v, lens, parents)
+            else:
+                r.check(ctx.prefill_packed(0, r.slots, r.rows, lens, *gpu(q, k, v)), q, k, v, lens)
+
+
 @pytest.mark.parametrize("shape,nodes", [("l8b", 1), ("l8b", 2), ("g2_64", 1), ("l70b", 1)])
 def test_one_long_sequence_among_short_ones(cuda, shape, nodes):
     """Splits of the long one, more blocks than run at once; it comes last."""
