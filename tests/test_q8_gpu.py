@@ -701,6 +701,39 @@ def test_decode_of_items_in_many_parts(cuda):
             np.testing.assert_array_equal(vv, vn)
 
 
+def test_call_after_a_replay_that_wrote_its_layer(cuda):
+    """The last eager call before the replay was on the other layer."""
+    import torch
+    rng = np.random.default_rng(39)
+    with make("l8b", 1200, max_batch=4, n_layers=2) as ctx:
+        stream = torch.cuda.Stream()
+        ctx.bind_torch_stream(stream)
+        rs = [Ragged(ctx, rng, range(4), [1023, 500, 31, 0], layer=x) for x in (0, 1)]
+        q, k, v = rs[0].inputs([1] * 4)
+        dev = gpu(q, k, v)
+        with torch.cuda.stream(stream):
+            ctx.decode_batched(1, rs[1].slots, rs[1].rows, *dev)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            first = ctx.decode_batched(0, rs[0].slots, rs[0].rows, *dev)
+        q2, k2, v2 = rs[0].inputs([1] * 4)
+        dev2 = gpu(q2, k2, v2)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            ctx.decode_batched(1, rs[1].slots, rs[1].rows, *dev)
+            graph.replay()
+            second = ctx.decode_batched(0, rs[0].slots, rs[0].rows + 1, *dev2)
+        torch.cuda.synchronize()
+        for i in range(4):
+            sl = slice(i, i + 1)
+            ref, kn, vn = attend(ctx, rs[0].k[i], rs[0].v[i], q[sl], k[sl], v[sl])
+            near(first.cpu().numpy()[sl], ref)
+            ref, _, _ = attend(ctx, np.concatenate([rs[0].k[i], kn]), np.concatenate([rs[0].v[i], vn]), q2[sl], k2[sl], v2[sl])
+            near(second.cpu().numpy()[sl], ref)
+        del graph
+
+
 @pytest.mark.parametrize("shape", ["mha128", "mha64", "g2_64"])
 @pytest.mark.parametrize("drafted", [False, True])
 def test_new_rows_that_few_or_many_warps_store(cuda, shape, drafted):
