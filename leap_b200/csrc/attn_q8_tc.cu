@@ -813,17 +813,40 @@ int launch_tc_g(leap_ctx *c, const TcArgs &a, const Q8Seqs &tab, const Q8TcPlan 
 }
 
 // A block's work apart from its tiles (queries, first loads, output) costs
-// about as much as this many tiles, the join of splits as two and 1.5 for every 16
+// about as much as kOverhead tiles, the join of splits as two and one for every 16
 // of a tile, whose loads are in flight together.
-constexpr long kOverhead = 6, kJoinSplits = 16;
+constexpr long kOverhead = 5, kJoinSplits = 16;
 
-// Sequences longest first, and the tiles of a split.  Blocks are handed to SMs as
-// they fall free: one wave takes as long as its longest block; more take all work /
-// SMs and part of a block at the end, and no less than the waves of full splits.
-// The chunk with the least of that is taken, among those whose partials fit the
-// scratch.  Its choice is within 7% of the best chunk in 45 batches (1 to 64
-// sequences, 300 to 32768 rows, 16 to 4096 new; with 3, one join of 2 and without the
-// waves up to 26% off: 16 on 2048 rows 19.1 us, now 15.2).
+// Blocks as the hardware hands them out, in order, each to the SM that is free first:
+// how long all take.  Loads are kept as counts of SMs; those of a ring differ by one
+// block at most.
+struct Schedule {
+    static constexpr int kRing = 1024;
+    int free_at[kRing] = {};  // SMs that fall free at a time, modulo kRing
+    long now = 0, end = 0;
+    int unit;                 // tiles of a time step
+
+    Schedule(int sms, int longest) : unit((longest + int(kOverhead)) / (kRing - 8) + 1) { free_at[0] = sms; }
+    void put(long blocks, int tiles) {
+        const int t = (tiles + int(kOverhead) + unit - 1) / unit;
+        while (blocks > 0) {
+            while (free_at[now % kRing] == 0) ++now;
+            const int k = int(std::min(blocks, long(free_at[now % kRing])));
+            free_at[now % kRing] -= k;
+            free_at[(now + t) % kRing] += k;
+            blocks -= k;
+            end = std::max(end, now + t);
+        }
+    }
+    long time() const { return end * unit; }
+};
+constexpr int kScheduleTiles = 128;  // query tiles up to which it is worked out (host time)
+
+// Sequences longest first, and the tiles of a split: the chunk that takes least, by
+// Schedule, or for many query tiles by all work / SMs and part of a block at the end,
+// among those whose partials fit the scratch.  Device us with all work / SMs alone and
+// so: 8 ragged trees (64/8x128) 97, 87; 16 nodes each on one of 32768 and 19 of 300 rows
+// 71, 61; 16 nodes on 2048 rows 19.1, 15.5; of 75 batches one lost (6%).
 void plan_tc(const leap_ctx *c, const Q8Seqs &tab, bool tree, Q8TcPlan &plan) {
     const int bt = kBM / c->group;
     plan.n = 0;
@@ -840,24 +863,43 @@ void plan_tc(const leap_ctx *c, const Q8Seqs &tab, bool tree, Q8TcPlan &plan) {
         mean[i] = tree ? all[i] : (all[i] + unsigned(tab.pos[s] + bt + kBN - 1) / kBN + 1) / 2;
     }
     const int longest = plan.n ? int(all[0]) : 1;
+    long n_tiles = 0;
+    for (int i = 0; i < plan.n; ++i) n_tiles += plan.n_qt[i];
     long best = -1;
     plan.chunk = longest;
     for (int chunk = longest; chunk >= 1; chunk -= std::max(chunk / 16, 1)) {
-        long work = 0, parts = 0, items = 0, full = 0;
+        long work = 0, parts = 0, items = 0;
         for (int i = 0; i < plan.n; ++i) {
             const unsigned ns = (all[i] + chunk - 1) / chunk;
             work += plan.n_qt[i] * (mean[i] + ns * kOverhead);
             if (ns > 1) parts += plan.n_qt[i] * long(ns);
             items += plan.n_qt[i] * long(ns);
-            full += plan.n_qt[i] * long(mean[i] / chunk);
         }
         if (parts * c->n_kv > c->q8_tc_parts) break;
         const long block = chunk + kOverhead, sms = c->num_sms;
-        const bool wave = items * c->n_kv <= sms;
-        const long waves = std::max((full * c->n_kv + sms - 1) / sms, 1L);
         const long splits = (longest + chunk - 1) / chunk;
-        const long cost = (wave ? 10 * block : std::max(10 * work * c->n_kv / sms + 3 * block, 10 * waves * block)) +
-                          (parts ? 20 + 15 * ((splits + kJoinSplits - 1) / kJoinSplits) : 0);  // tenths of a tile
+        const long join = parts ? 2 + (splits + kJoinSplits - 1) / kJoinSplits : 0, mean_load = work * c->n_kv / sms;
+        long cost = join + block;
+        if (items * c->n_kv > sms) {
+            if (n_tiles > kScheduleTiles) {
+                cost = join + std::max(mean_load + block / 4, block);
+            } else {
+                if (best >= 0 && join + std::max(mean_load, block) >= best) continue;
+                Schedule when(c->num_sms, longest);
+                for (int i = 0; i < plan.n; ++i) {
+                    const int s = plan.seq[i], n = tab.tok0[s + 1] - tab.tok0[s];
+                    const int ns = int(all[i] + chunk - 1) / chunk;
+                    for (int qt = plan.n_qt[i] - 1; qt >= 0; --qt) {
+                        const int tiles = tree ? int(all[i]) : (tab.pos[s] + std::min((qt + 1) * bt, n) + kBN - 1) / kBN;
+                        const int full = tiles / chunk, rest = full < ns;
+                        when.put(long(full) * c->n_kv, chunk);
+                        if (rest) when.put(c->n_kv, tiles - full * chunk);
+                        when.put(long(ns - full - rest) * c->n_kv, 0);  // splits that this tile does not see
+                    }
+                }
+                cost = join + when.time();
+            }
+        }
         if (best < 0 || cost < best) {
             best = cost;
             plan.chunk = chunk;
