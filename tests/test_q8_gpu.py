@@ -701,6 +701,23 @@ def test_decode_of_items_in_many_parts(cuda):
             np.testing.assert_array_equal(vv, vn)
 
 
+@pytest.mark.parametrize("shape,drafted", [("l8b", True), ("l8b", False), ("mha64", True), ("l70b", False)])
+def test_one_long_sequence_among_short_ones_on_tensor_cores(cuda, shape, drafted):
+    """Splits of unequal sequences, with query tiles that do not see the last of them."""
+    rng = np.random.default_rng(40)
+    lens = [16] * 18 + [100, 70]
+    with make(shape, 5000, max_batch=20) as ctx:
+        rows = rng.integers(0, 400, 20)
+        rows[-2:] = [0, 4900]
+        r = Ragged(ctx, rng, rng.permutation(20), rows)
+        q, k, v = r.inputs(lens)
+        if drafted:
+            parents = np.concatenate([tree(rng, n) for n in lens])
+            r.check(ctx.decode_tree(0, r.slots, r.rows, lens, parents, *gpu(q, k, v)), q, k, v, lens, parents)
+        else:
+            r.check(ctx.prefill_packed(0, r.slots, r.rows, lens, *gpu(q, k, v)), q, k, v, lens)
+
+
 def test_call_after_a_replay_that_wrote_its_layer(cuda):
     """The last eager call before the replay was on the other layer."""
     import torch
