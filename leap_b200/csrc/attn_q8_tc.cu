@@ -740,9 +740,7 @@ q8_tc_join_kernel(const TcArgs a, const __grid_constant__ Q8Seqs tab, const __gr
 #pragma unroll
         for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
         top = fmaxf(top, mx);
-        const float back = mx == -INFINITY ? 0.f : fast_exp2(mx - top);
-        // a split that had nothing this row sees weighs nothing
-        const float e = y.x == -INFINITY ? 0.f : fast_exp2(y.x - top);
+        const float back = part_weight(mx, top), e = part_weight(y.x, top);
         float part = y.y * e;
 #pragma unroll
         for (int off = 16; off >= 1; off >>= 1) part += __shfl_xor_sync(0xffffffffu, part, off);
@@ -753,7 +751,7 @@ q8_tc_join_kernel(const TcArgs a, const __grid_constant__ Q8Seqs tab, const __gr
 #pragma unroll
             for (int k = 0; k < U; ++k) {
                 const float w = __shfl_sync(0xffffffffu, e, (s1 + k - s0) & 31);
-                if (s1 + k >= ns || w == 0.f) continue;
+                if (s1 + k >= ns) continue;
                 v.x += z[k].x * w; v.y += z[k].y * w; v.z += z[k].z * w; v.w += z[k].w * w;
             }
             s1 += U;

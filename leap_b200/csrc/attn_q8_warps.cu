@@ -276,14 +276,14 @@ q8_warps_kernel(const __grid_constant__ RowsArgs a, const __grid_constant__ Q8Se
                         float top = mx;
 #pragma unroll
                         for (int k = 0; k < U; ++k) top = fmaxf(top, y[k].x);
-                        const float back = mx == -INFINITY ? 0.f : fast_exp2(mx - top);
+                        const float back = part_weight(mx, top);
                         mx = top;
                         sum *= back;
                         v.x *= back; v.y *= back; v.z *= back; v.w *= back;
 #pragma unroll
                         for (int k = 0; k < U; ++k) {
-                            if (y[k].x == -INFINITY) continue;
-                            const float e = fast_exp2(y[k].x - top);
+                            if (s0 + k >= ns) continue;
+                            const float e = part_weight(y[k].x, top);
                             sum += y[k].y * e;
                             v.x += z[k].x * e; v.y += z[k].y * e; v.z += z[k].z * e; v.w += z[k].w * e;
                         }
