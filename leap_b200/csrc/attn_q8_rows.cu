@@ -216,7 +216,7 @@ q8_rows_kernel(const RowsArgs a, const __grid_constant__ Q8Seqs tab,
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-            const float e = part_weight(s_m[w][r], mx);
+            const float e = s_m[w][r] == -INFINITY ? 0.f : fast_exp2(s_m[w][r] - mx);
             const float4 x = *reinterpret_cast<const float4 *>(s_o + (w * kQ8Rows + r) * HD + d);
             sum += s_l[w][r] * e;
             v.x += x.x * e; v.y += x.y * e; v.z += x.z * e; v.w += x.w * e;
@@ -228,7 +228,7 @@ q8_rows_kernel(const RowsArgs a, const __grid_constant__ Q8Seqs tab,
         } else {
             const size_t p = (part0 + split) * kQ8Rows + r;
             *reinterpret_cast<float4 *>(a.part_o + p * HD + d) = v;
-            if (d == 0) *reinterpret_cast<float2 *>(a.part_ml + 2 * p) = make_float2(mx, sum);
+            if (d == 0) *reinterpret_cast<float2 *>(a.part_ml + 2 * p) = make_float2(part_max(mx, sum), sum);
         }
     }
     if (nsplit == 1) return;
@@ -264,14 +264,14 @@ q8_rows_kernel(const RowsArgs a, const __grid_constant__ Q8Seqs tab,
             float top = mx;
 #pragma unroll
             for (int k = 0; k < U; ++k) top = fmaxf(top, y[k].x);
-            const float back = part_weight(mx, top);
+            const float back = mx == -INFINITY ? 0.f : fast_exp2(mx - top);
             mx = top;
             sum *= back;
             v.x *= back; v.y *= back; v.z *= back; v.w *= back;
 #pragma unroll
             for (int k = 0; k < U; ++k) {
-                if (s0 + k * ng >= nsplit) continue;
-                const float e = part_weight(y[k].x, top);
+                if (y[k].x == -INFINITY) continue;
+                const float e = fast_exp2(y[k].x - top);
                 sum += y[k].y * e;
                 v.x += z[k].x * e; v.y += z[k].y * e; v.z += z[k].z * e; v.w += z[k].w * e;
             }
@@ -282,15 +282,16 @@ q8_rows_kernel(const RowsArgs a, const __grid_constant__ Q8Seqs tab,
         float2 *s_y = reinterpret_cast<float2 *>(smem + 32 * W * 16);
         if (grp < ng) {
             s_v[tid] = v;
-            s_y[tid] = make_float2(mx, sum);
+            s_y[tid] = make_float2(part_max(mx, sum), sum);
         }
         __syncthreads();
         if (grp == 0)
             for (int k = 1; k < ng; ++k) {
                 const float4 z = s_v[k * items + f];
                 const float2 y = s_y[k * items + f];
+                if (y.x == -INFINITY) continue;
                 const float top = fmaxf(mx, y.x);
-                const float e0 = part_weight(mx, top), e1 = part_weight(y.x, top);
+                const float e0 = mx == -INFINITY ? 0.f : fast_exp2(mx - top), e1 = fast_exp2(y.x - top);
                 mx = top;
                 sum = sum * e0 + y.y * e1;
                 v.x = v.x * e0 + z.x * e1; v.y = v.y * e0 + z.y * e1;

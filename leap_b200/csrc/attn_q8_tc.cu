@@ -740,7 +740,10 @@ q8_tc_join_kernel(const TcArgs a, const __grid_constant__ Q8Seqs tab, const __gr
 #pragma unroll
         for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
         top = fmaxf(top, mx);
-        const float back = part_weight(mx, top), e = part_weight(y.x, top);
+        const float back = mx == -INFINITY ? 0.f : fast_exp2(mx - top);
+        // a split that had nothing this row sees weighs nothing; its sums are taken in
+        // all the same (zeros, or the NaN that it saw)
+        const float e = y.x == -INFINITY ? 0.f : fast_exp2(y.x - top);
         float part = y.y * e;
 #pragma unroll
         for (int off = 16; off >= 1; off >>= 1) part += __shfl_xor_sync(0xffffffffu, part, off);

@@ -244,7 +244,7 @@ q8_warps_kernel(const __grid_constant__ RowsArgs a, const __grid_constant__ Q8Se
                 *reinterpret_cast<float4 *>(d + HD / 8 + i) =
                     make_float4(o[i][1] * by, o[i + 1][1] * by, o[i + 2][1] * by, o[i + 3][1] * by);
             }
-            if (ns > 1 && t == 0) *reinterpret_cast<float2 *>(a.part_ml + 2 * p) = make_float2(m, l);
+            if (ns > 1 && t == 0) *reinterpret_cast<float2 *>(a.part_ml + 2 * p) = make_float2(part_max(m, l), l);
         }
         if (ns > 1) {
             __threadfence();
@@ -276,14 +276,14 @@ q8_warps_kernel(const __grid_constant__ RowsArgs a, const __grid_constant__ Q8Se
                         float top = mx;
 #pragma unroll
                         for (int k = 0; k < U; ++k) top = fmaxf(top, y[k].x);
-                        const float back = part_weight(mx, top);
+                        const float back = mx == -INFINITY ? 0.f : fast_exp2(mx - top);
                         mx = top;
                         sum *= back;
                         v.x *= back; v.y *= back; v.z *= back; v.w *= back;
 #pragma unroll
                         for (int k = 0; k < U; ++k) {
-                            if (s0 + k >= ns) continue;
-                            const float e = part_weight(y[k].x, top);
+                            if (y[k].x == -INFINITY) continue;
+                            const float e = fast_exp2(y[k].x - top);
                             sum += y[k].y * e;
                             v.x += z[k].x * e; v.y += z[k].y * e; v.z += z[k].z * e; v.w += z[k].w * e;
                         }
