@@ -141,6 +141,7 @@ q8_rows_kernel(const RowsArgs a, const __grid_constant__ Q8Seqs tab,
 #pragma unroll
     for (int i = 0; i < M::NT; ++i) o[i][0] = o[i][1] = 0.f;
 
+    ScaleSpan span;
     bool ok = true;
     int tile = 0;
     for (; tile < n_tiles; ++tile) {
@@ -152,16 +153,15 @@ q8_rows_kernel(const RowsArgs a, const __grid_constant__ Q8Seqs tab,
         const int n = row1 - (row0 + (warp + tile * W) * kTile);  // rows of it that are cached
         float s[kTile / 8][2];
         M::scores(st, sks, s_q, fac, s);
-        float sv = svs[lane];
         if (n < kTile) {
-            if (lane >= n) sv = 0.f;
 #pragma unroll
             for (int j = 0; j < kTile / 8; ++j) {
                 if (8 * j + 2 * t >= n) s[j][0] = -INFINITY;
                 if (8 * j + 2 * t + 1 >= n) s[j][1] = -INFINITY;
             }
         }
-        M::absorb(st + kTile * HD, svs, top_scale(sv), s, m, l, o);
+        const float top = span.take(svs[lane], lane < n);
+        M::absorb(st + kTile * HD, svs, top, span.wide(), s, m, l, o);
         __syncwarp();  // the buffer is free
         if (asked < n_tiles) {
             if (lane == 0) request(asked);
@@ -183,7 +183,8 @@ q8_rows_kernel(const RowsArgs a, const __grid_constant__ Q8Seqs tab,
                 const int key = 8 * j + 2 * t + e;
                 if (mine >= n_new || !see.sees(t0, mine, key)) s[j][e] = -INFINITY;
             }
-        N::absorb(s_new + kNew * HD, s_nvs, top_scale(lane < kNew ? s_nvs[lane] : 0.f), s, m, l, o);
+        const float top = span.take(lane < kNew ? s_nvs[lane] : 0.f, lane < n_new);
+        N::absorb(s_new + kNew * HD, s_nvs, top, span.wide(), s, m, l, o);
     }
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);

@@ -9,7 +9,7 @@
 // tile, head r % G of the kv head's group) and a range of key tiles of 128.
 //
 // Arithmetic: codes are exact in FP16.  Queries (scaled by a power of two for
-// each row) and weights p*s_v (by one for each tile) are split into two FP16,
+// each row) and weights p*s_v (by one for each tile, or row and tile) are split into two FP16,
 // hi + lo, 22 bits: two FP16 products in place of one give FP32-like results,
 // and are what bounds the kernel (twice the FLOPs of one FP16 product; 32
 // tcgen05.mma of 128x128x16 a tile, about 2048 cycles).  Tensor-core sums are
@@ -154,7 +154,8 @@ q8_tc_kernel(const __grid_constant__ TcArgs a, const __grid_constant__ Q8Seqs ta
     extern __shared__ unsigned char smem_raw[];
     __shared__ TcBars bars;
     __shared__ __align__(16) float s_ks[kSlots][kBN], s_vs[kSlots][kBN];
-    __shared__ float s_vdown[kSlots], s_fac[kBM], s_mx[2][2][kBM], s_l[2][kBM];
+    __shared__ float s_vdown[kSlots];  // negative: wide (ScaleSpan)
+    __shared__ float s_fac[kBM], s_mx[2][2][kBM], s_most[2][2][kBM], s_l[2][kBM];
     __shared__ int8_t s_parent[TREE ? kMaxTreeNodes : 1];
     __shared__ uint32_t s_anc[TREE ? 4 : 1][kBM];  // TREE: what each row sees of the run
     __shared__ uint32_t tmem_sh;
@@ -434,6 +435,8 @@ q8_tc_kernel(const __grid_constant__ TcArgs a, const __grid_constant__ Q8Seqs ta
             const float ref = mn == -INFINITY ? 0.f : mn;  // nothing seen so far
             const float al = fast_exp2(m - ref);
             m = mn;
+            float vd = s_vdown[slot];
+            float2 up2 = make_float2(1.f, 1.f);
             const float2 fac2 = make_float2(fac, fac), nref2 = make_float2(-ref, -ref);
             float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
             // s becomes p a step of 16 keys (one of the PV product) ahead of the
@@ -461,7 +464,7 @@ q8_tc_kernel(const __grid_constant__ TcArgs a, const __grid_constant__ Q8Seqs ta
                     for (int i = 0; i < 8; ++i) {
                         const float4 g = vs[4 * c + i / 2];
                         const float2 p = make_float2(s[c][2 * i], s[c][2 * i + 1]);
-                        float2 w = __fmul2_rn(p, i & 1 ? make_float2(g.z, g.w) : make_float2(g.x, g.y));
+                        float2 w = __fmul2_rn(FULL ? p : __fmul2_rn(p, up2), i & 1 ? make_float2(g.z, g.w) : make_float2(g.x, g.y));
                         if (!FULL) {  // what is not seen (p = 0) takes no part, whatever its scale
                             if (off[c] >> (2 * i) & 1) w.x = 0.f;
                             if (off[c] >> (2 * i + 1) & 1) w.y = 0.f;
@@ -478,10 +481,35 @@ q8_tc_kernel(const __grid_constant__ TcArgs a, const __grid_constant__ Q8Seqs ta
                     tc::st16u_free(scol + 16 * c, hl);
                 }
             };
-            if (full) weights(std::true_type());
-            else weights(std::false_type());
+            if (full && vd > 0.f) {
+                weights(std::true_type());
+            } else {
+                if (vd < 0.f) {
+                    // Scales far apart (every thread's vd says so): the unit is that of the
+                    // row's largest weight, known to a factor of two from its scores and
+                    // the scales' exponents.
+                    float most = -INFINITY;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int i = 0; i < 16; i += 4) {
+                            const float4 g = vs[4 * c + i / 4];
+                            const float gs[4] = {g.x, g.y, g.z, g.w};
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if (gs[e] > 0.f)
+                                    most = fmaxf(most, fmaf(s[c][i + e], fac, float(int(__float_as_uint(gs[e]) >> 23) - 127)));
+                        }
+                    s_most[b][half][row] = most;
+                    (void)group_and(true);
+                    most = fmaxf(most, s_most[b][half ^ 1][row]);
+                    const int u = most == -INFINITY ? 0 : int(fminf(fmaxf(14.f - ceilf(most - ref), -1.f), 120.f));
+                    up2.x = up2.y = __uint_as_float(uint32_t(127 + u) << 23);
+                    vd *= -__uint_as_float(uint32_t(127 - u) << 23);
+                }
+                weights(std::false_type());
+            }
             l = l * al + ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
-            const float vd = s_vdown[slot];
             tc::wait_st();
             // O(j-1), whose product ran beside this softmax; then PV(j) may start
             if (j > 0) ok = absorb(j - 1, alpha, vdown, s);
@@ -564,6 +592,7 @@ q8_tc_kernel(const __grid_constant__ TcArgs a, const __grid_constant__ Q8Seqs ta
                 *reinterpret_cast<uint4 *>(d1 + i * kStep) = expand(x.z, x.w);
             }
         };
+        ScaleSpan span;
         bool ok = true, awaited = a.k_new == nullptr;
         // before the first load of a tile that has rows of the run
         auto settle = [&](int j) {
@@ -585,18 +614,17 @@ q8_tc_kernel(const __grid_constant__ TcArgs a, const __grid_constant__ Q8Seqs ta
             // PV(j-4), that after the softmax of tile j-4.
             {
                 const int first = (j0 + j) * kBN, n = kv_end - first;
-                float top = 0.f;
+                uint32_t t = 0u, l = 0x7f7fffffu;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int r = 32 * i + lane;
-                    const float x = r < n ? gvs[first + r] : 0.f;
-                    top = fmaxf(top, x < INFINITY ? x : 0.f);
+                    ScaleSpan::look(r < n ? gvs[first + r] : 0.f, r < n, t, l);
                 }
-                const int e = max(int(__reduce_max_sync(0xffffffffu, __float_as_uint(top)) >> 23), 15);
+                const int e = max(int(__float_as_uint(span.take(t, l)) >> 23), 15);
                 const float vup = __uint_as_float(uint32_t(268 - e) << 23);
                 s_ks[slot][ct] = ct < n ? gks[first + ct] : 0.f;
                 s_vs[slot][ct] = ct < n ? gvs[first + ct] * vup : 0.f;
-                if (ct == 0) s_vdown[slot] = __uint_as_float(uint32_t(e - 14) << 23);
+                if (ct == 0) s_vdown[slot] = __uint_as_float(uint32_t(e - 14) << 23 | (span.wide() ? 0x80000000u : 0u));
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bars.sc_full[slot]);
             }
