@@ -367,8 +367,22 @@ LEAP_API int leap_engine_synthetic(const leap_model_config *cfg,
                                    float rope_theta, int max_chunk,
                                    leap_engine **out);
 
+/* The same with a choice of how the KV cache keeps its rows
+ * (leap_ctx_create_kv); the two above keep them as LEAP_KV_F32.  Only the
+ * cache asked for is ever allocated. */
+LEAP_API int leap_engine_open_kv(const char *path, int device, int layer_begin,
+                                 int layer_end, float rope_theta, int max_chunk,
+                                 int kv_kind, leap_engine **out);
+LEAP_API int leap_engine_synthetic_kv(const leap_model_config *cfg,
+                                      unsigned long long seed, int device,
+                                      int layer_begin, int layer_end,
+                                      float rope_theta, int max_chunk,
+                                      int kv_kind, leap_engine **out);
+
 /* Replace the engine's KV cache by an empty one that keeps its rows as
- * `kv_kind` says (leap_ctx_create_kv); engines are made with LEAP_KV_F32. */
+ * `kv_kind` says.  Both caches are there for a moment; on an error the engine
+ * keeps the one it had.  CUDA graphs captured from the engine before hold the
+ * old cache: capture them again. */
 LEAP_API int leap_engine_set_kv(leap_engine *e, int kv_kind);
 
 LEAP_API int leap_engine_destroy(leap_engine *e);

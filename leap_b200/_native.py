@@ -94,6 +94,11 @@ SIGNATURES: dict[str, tuple] = {
     "leap_engine_synthetic": (c_int, [ctypes.POINTER(ModelConfigC), ctypes.c_ulonglong, c_int,
                                       c_int, c_int, ctypes.c_float, c_int,
                                       ctypes.POINTER(c_void_p)]),
+    "leap_engine_open_kv": (c_int, [ctypes.c_char_p, c_int, c_int, c_int, ctypes.c_float, c_int,
+                                    c_int, ctypes.POINTER(c_void_p)]),
+    "leap_engine_synthetic_kv": (c_int, [ctypes.POINTER(ModelConfigC), ctypes.c_ulonglong, c_int,
+                                         c_int, c_int, ctypes.c_float, c_int, c_int,
+                                         ctypes.POINTER(c_void_p)]),
     "leap_engine_set_kv": (c_int, [c_void_p, c_int]),
     "leap_engine_destroy": (c_int, [c_void_p]),
     "leap_engine_config": (c_int, [c_void_p, ctypes.POINTER(ModelConfigC), c_int_p, c_int_p]),

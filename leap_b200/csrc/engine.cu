@@ -215,7 +215,7 @@ int allocate(leap_engine *e) {
 
 // The engine's attention context, made (again) with a cache of kv_kind.  The
 // one it had goes only once the new one is there.
-int make_attention(leap_engine *e, float theta, int kv_kind = LEAP_KV_F32) {
+int make_attention(leap_engine *e, float theta, int kv_kind) {
     const leap_model_config &c = e->cfg;
     std::vector<float> rc(size_t(c.seq_len) * (e->head_dim / 2)), rs(rc.size());
     ETRY(leap_rope_table(c.seq_len, e->head_dim, theta, rc.data(), rs.data()));
@@ -244,6 +244,12 @@ int make_attention(leap_engine *e, float theta, int kv_kind = LEAP_KV_F32) {
     e->device_bytes += b;
     e->rope_theta = theta;
     return LEAP_OK;
+}
+
+int check_kv_kind(int kv_kind) {
+    if (kv_kind == LEAP_KV_F32 || kv_kind == LEAP_KV_Q8) return LEAP_OK;
+    leap::set_error("kv kind %d unknown (LEAP_KV_F32 or LEAP_KV_Q8)", kv_kind);
+    return LEAP_ERR_INVALID;
 }
 
 int begin(leap_engine **out, const leap_model_config &cfg, int device, int lb, int le,
@@ -568,12 +574,19 @@ extern "C" {
 
 int leap_engine_open(const char *path, int device, int layer_begin, int layer_end,
                      float rope_theta, int max_chunk, leap_engine **out) {
+    return leap_engine_open_kv(path, device, layer_begin, layer_end, rope_theta, max_chunk,
+                               LEAP_KV_F32, out);
+}
+
+int leap_engine_open_kv(const char *path, int device, int layer_begin, int layer_end,
+                        float rope_theta, int max_chunk, int kv_kind, leap_engine **out) {
     leap::clear_error();
     if (!path || !out) {
         leap::set_error("null argument");
         return LEAP_ERR_INVALID;
     }
     *out = nullptr;
+    ETRY(check_kv_kind(kv_kind));
     Mapped m;
     m.fd = open(path, O_RDONLY);
     if (m.fd < 0) {
@@ -605,7 +618,7 @@ int leap_engine_open(const char *path, int device, int layer_begin, int layer_en
         Cursor cur{b + hdr, b + m.size};
         st = cfg.quantized ? load_q8(e, cur) : load_fp32(e, cur);
     }
-    if (st == LEAP_OK) st = make_attention(e, rope_theta > 0.f ? rope_theta : 500000.f);
+    if (st == LEAP_OK) st = make_attention(e, rope_theta > 0.f ? rope_theta : 500000.f, kv_kind);
     if (st != LEAP_OK) {
         free_engine(e);
         return st;
@@ -617,17 +630,26 @@ int leap_engine_open(const char *path, int device, int layer_begin, int layer_en
 int leap_engine_synthetic(const leap_model_config *cfg, unsigned long long seed, int device,
                           int layer_begin, int layer_end, float rope_theta, int max_chunk,
                           leap_engine **out) {
+    return leap_engine_synthetic_kv(cfg, seed, device, layer_begin, layer_end, rope_theta,
+                                    max_chunk, LEAP_KV_F32, out);
+}
+
+int leap_engine_synthetic_kv(const leap_model_config *cfg, unsigned long long seed, int device,
+                             int layer_begin, int layer_end, float rope_theta, int max_chunk,
+                             int kv_kind, leap_engine **out) {
     leap::clear_error();
     if (!cfg || !out) {
         leap::set_error("null argument");
         return LEAP_ERR_INVALID;
     }
+    *out = nullptr;
+    ETRY(check_kv_kind(kv_kind));
     DevGuard g(device);
     leap_engine *e = nullptr;
     int st = begin(out, *cfg, device, layer_begin, layer_end, max_chunk, &e);
     if (st == LEAP_OK) st = allocate(e);
     if (st == LEAP_OK) st = synthesize(e, seed);
-    if (st == LEAP_OK) st = make_attention(e, rope_theta > 0.f ? rope_theta : 500000.f);
+    if (st == LEAP_OK) st = make_attention(e, rope_theta > 0.f ? rope_theta : 500000.f, kv_kind);
     if (st != LEAP_OK) {
         free_engine(e);
         return st;
@@ -638,10 +660,11 @@ int leap_engine_synthetic(const leap_model_config *cfg, unsigned long long seed,
 
 int leap_engine_set_kv(leap_engine *e, int kv_kind) {
     leap::clear_error();
-    if (!e || (kv_kind != LEAP_KV_F32 && kv_kind != LEAP_KV_Q8)) {
-        leap::set_error("engine set_kv: null engine or unknown kv kind %d", kv_kind);
+    if (!e) {
+        leap::set_error("null engine");
         return LEAP_ERR_INVALID;
     }
+    ETRY(check_kv_kind(kv_kind));
     DevGuard g(e->device);
     return make_attention(e, e->rope_theta, kv_kind);
 }

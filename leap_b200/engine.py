@@ -13,7 +13,7 @@ import ctypes
 
 import numpy as np
 
-from ._native import LEAP_KV_F32, LeapError, ModelConfigC, check, lib
+from ._native import LeapError, ModelConfigC, check, lib
 from .attention import kv_kind
 from .modelfile import ModelConfig
 
@@ -48,34 +48,33 @@ class Transformer:
                layer_range=None, max_chunk: int = 512, kv: str = "f32") -> "Transformer":
         """Transformer::create (src/inference/TransformerFactory.cpp:59).
         ``kv``: how cached rows are kept (``"f32"`` or ``"q8"``, 8 bits)."""
+        kind = kv_kind(kv)
         lb, le = layer_range if layer_range is not None else (0, -1)
         h = ctypes.c_void_p()
-        check(lib().leap_engine_open(checkpoint_path.encode(), device, lb, le,
-                                     ctypes.c_float(rope_theta), max_chunk, ctypes.byref(h)))
-        return Transformer(h)._with_kv(kv)
+        check(lib().leap_engine_open_kv(checkpoint_path.encode(), device, lb, le,
+                                        ctypes.c_float(rope_theta), max_chunk, kind,
+                                        ctypes.byref(h)))
+        return Transformer(h)
 
     @staticmethod
     def synthetic(config: ModelConfig, quantized: bool, seed: int = 0, group_size: int = 64,
                   device: int = 0, rope_theta: float = 0.0, layer_range=None,
                   max_chunk: int = 512, kv: str = "f32") -> "Transformer":
         """N(0, 0.02) weights generated on the device (no file)."""
+        kind = kv_kind(kv)
         lb, le = layer_range if layer_range is not None else (0, -1)
         c = ModelConfigC(*config.as_tuple(), int(quantized), group_size if quantized else 0, 1)
         h = ctypes.c_void_p()
-        check(lib().leap_engine_synthetic(ctypes.byref(c), seed, device, lb, le,
-                                          ctypes.c_float(rope_theta), max_chunk,
-                                          ctypes.byref(h)))
-        return Transformer(h)._with_kv(kv)
-
-    def _with_kv(self, kv: str) -> "Transformer":
-        if kv_kind(kv) != LEAP_KV_F32:
-            self.set_kv(kv)
-        return self
+        check(lib().leap_engine_synthetic_kv(ctypes.byref(c), seed, device, lb, le,
+                                             ctypes.c_float(rope_theta), max_chunk, kind,
+                                             ctypes.byref(h)))
+        return Transformer(h)
 
     def set_kv(self, kv: str) -> None:
         """Replace the KV cache by an empty one whose rows are kept as ``kv``
         says: ``"f32"``, or ``"q8"`` (a byte a value, about a quarter of the
-        memory and of the bytes a decode step reads)."""
+        memory and of the bytes a decode step reads).  Both are allocated for
+        a moment; ``create(..., kv="q8")`` allocates the one alone."""
         check(lib().leap_engine_set_kv(self.handle, kv_kind(kv)))
 
     def close(self) -> None:
