@@ -380,8 +380,9 @@ LEAP_API int leap_engine_synthetic_kv(const leap_model_config *cfg,
                                       int kv_kind, leap_engine **out);
 
 /* Replace the engine's KV cache by an empty one that keeps its rows as
- * `kv_kind` says.  Both caches are there for a moment; on an error the engine
- * keeps the one it had.  CUDA graphs captured from the engine before hold the
+ * `kv_kind` says.  Waits for the engine's work, whose errors it returns
+ * (leap_engine_sync).  Both caches are there for a moment; on an error the
+ * engine keeps the one it had.  CUDA graphs captured from the engine before hold the
  * old cache: capture them again. */
 LEAP_API int leap_engine_set_kv(leap_engine *e, int kv_kind);
 

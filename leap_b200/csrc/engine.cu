@@ -666,6 +666,7 @@ int leap_engine_set_kv(leap_engine *e, int kv_kind) {
     }
     ETRY(check_kv_kind(kv_kind));
     DevGuard g(e->device);
+    ETRY(leap_engine_sync(e));  // an error found on the device goes with the old context
     return make_attention(e, e->rope_theta, kv_kind);
 }
 

@@ -64,3 +64,22 @@ def test_a_context_that_only_8_bit_rows_fit(cuda):
         assert t.device_bytes() < 0.4 * total
         out = t.forward(3, 0)
         assert np.isfinite(out).all()
+
+
+@pytest.mark.gpu
+def test_replacing_the_cache_reports_what_went_wrong_before(cuda):
+    """A token id outside the vocabulary, found on the device: the error is not
+    lost with the cache's context, and the engine keeps what it had."""
+    import torch
+    with Transformer.synthetic(CFG, False, seed=2) as t:
+        t.bind_torch_stream()
+        before = t.device_bytes()
+        want = t.forward(7, 0)
+        x = torch.empty(1, CFG.dim, device="cuda")
+        t.embed_device(torch.tensor([CFG.vocab_size], dtype=torch.int32, device="cuda"), x)
+        with pytest.raises(LeapError, match="token id"):
+            t.set_kv("q8")
+        assert t.device_bytes() == before
+        np.testing.assert_array_equal(t.forward(7, 0), want)
+        t.set_kv("q8")
+        assert t.device_bytes() != before
