@@ -232,16 +232,14 @@ int make_attention(leap_engine *e, float theta, int kv_kind) {
     d.rope_sin = rs.data();
     leap_ctx *fresh = nullptr;
     ETRY(leap_ctx_create_kv(&d, kv_kind, &fresh));
-    size_t b = 0;
     if (e->attn) {
-        leap_ctx_device_bytes(e->attn, &b);
-        e->device_bytes -= b;
+        e->device_bytes -= e->attn_bytes;
         leap_ctx_destroy(e->attn);  // waits for its stream
     }
     e->attn = fresh;
     ETRY(leap_ctx_set_stream(e->attn, e->stream));
-    leap_ctx_device_bytes(e->attn, &b);
-    e->device_bytes += b;
+    leap_ctx_device_bytes(e->attn, &e->attn_bytes);
+    e->device_bytes += e->attn_bytes;
     e->rope_theta = theta;
     return LEAP_OK;
 }

@@ -76,6 +76,7 @@ struct leap_engine {
     int device = 0;
     cudaStream_t own_stream = nullptr, stream = nullptr;
     leap_ctx *attn = nullptr;
+    size_t attn_bytes = 0;   // of device_bytes
     float rope_theta = 0.f;  // what attn's table was made with
 
     std::vector<void *> allocs;  // every device allocation, freed at destroy

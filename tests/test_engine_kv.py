@@ -83,3 +83,15 @@ def test_replacing_the_cache_reports_what_went_wrong_before(cuda):
         np.testing.assert_array_equal(t.forward(7, 0), want)
         t.set_kv("q8")
         assert t.device_bytes() != before
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("first,then", [("f32", "q8"), ("q8", "f32"), ("f32", "f32")])
+def test_device_bytes_after_a_replaced_cache(cuda, first, then):
+    """What prefill allocated beside the old cache is gone with it."""
+    with Transformer.synthetic(CFG, False, kv=then) as t:
+        want = t.device_bytes()
+    with Transformer.synthetic(CFG, False, kv=first) as t:
+        t.prefill(np.arange(100))
+        t.set_kv(then)
+        assert t.device_bytes() == want
