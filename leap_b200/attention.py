@@ -59,8 +59,14 @@ def kv_kind(kv: str) -> int:
 
 
 def _ints(a, name: str, n: int | None = None) -> np.ndarray:
-    """A 1-D host int32 array (kept as it is when it is one already)."""
-    a = np.ascontiguousarray(a, np.int32)
+    """A 1-D host int32 array (kept as it is when it is one already) of whole
+    numbers, none of which the conversion may change."""
+    a = np.asarray(a)
+    if a.dtype != np.int32:
+        if a.size and (a.dtype.kind not in "iu" or a.min() < -2**31 or a.max() >= 2**31):
+            raise ValueError(f"{name} must be whole numbers of 32 bits")
+        a = a.astype(np.int32)
+    a = np.ascontiguousarray(a)
     if a.ndim != 1 or (n is not None and a.shape[0] != n):
         raise ValueError(f"{name} must be 1-D" + ("" if n is None else f" of length {n}"))
     return a
