@@ -141,7 +141,6 @@ q8_rows_kernel(const RowsArgs a, const __grid_constant__ Q8Seqs tab,
 #pragma unroll
     for (int i = 0; i < M::NT; ++i) o[i][0] = o[i][1] = 0.f;
 
-    ScaleSpan span;
     bool ok = true;
     int tile = 0;
     for (; tile < n_tiles; ++tile) {
@@ -160,8 +159,7 @@ q8_rows_kernel(const RowsArgs a, const __grid_constant__ Q8Seqs tab,
                 if (8 * j + 2 * t + 1 >= n) s[j][1] = -INFINITY;
             }
         }
-        const float top = span.take(svs[lane], lane < n);
-        M::absorb(st + kTile * HD, svs, top, span.wide(), s, m, l, o);
+        M::absorb(st + kTile * HD, svs, s, m, l, o);
         __syncwarp();  // the buffer is free
         if (asked < n_tiles) {
             if (lane == 0) request(asked);
@@ -183,8 +181,7 @@ q8_rows_kernel(const RowsArgs a, const __grid_constant__ Q8Seqs tab,
                 const int key = 8 * j + 2 * t + e;
                 if (mine >= n_new || !see.sees(t0, mine, key)) s[j][e] = -INFINITY;
             }
-        const float top = span.take(lane < kNew ? s_nvs[lane] : 0.f, lane < n_new);
-        N::absorb(s_new + kNew * HD, s_nvs, top, span.wide(), s, m, l, o);
+        N::absorb(s_new + kNew * HD, s_nvs, s, m, l, o);
     }
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);

@@ -180,7 +180,6 @@ q8_warps_kernel(const __grid_constant__ RowsArgs a, const __grid_constant__ Q8Se
             }
         }
         __syncwarp();
-        ScaleSpan span;
         float m = -INFINITY, l = 0.f, o[M::NT][2];
 #pragma unroll
         for (int i = 0; i < M::NT; ++i) o[i][0] = o[i][1] = 0.f;
@@ -219,8 +218,7 @@ q8_warps_kernel(const __grid_constant__ RowsArgs a, const __grid_constant__ Q8Se
             ok = __all_sync(0xffffffffu, mbar_wait(&bars[warp][1], phase));
             if (!ok) break;
             const float *svs = reinterpret_cast<const float *>(buf + C::kHalf + kTile * HD);
-            const float top = span.take(svs[lane], lane < n + n_new);
-            M::absorb(buf + C::kHalf, svs, top, span.wide(), s, m, l, o);
+            M::absorb(buf + C::kHalf, svs, s, m, l, o);
             __syncwarp();
             if (more) ask(1);
             phase ^= 1;

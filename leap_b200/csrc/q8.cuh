@@ -154,41 +154,6 @@ __device__ __forceinline__ uint32_t q8_load_codes(const uint8_t *head, int r, in
     return *reinterpret_cast<const uint16_t *>(head + q8_chunk<HD>(r, lane >> 3) + (lane & 7) * 2);
 }
 
-// How far apart the V scales lie of the rows that a warp has taken so far, as
-// FP32 bits (scales are never negative; NaN counts for nothing).  FP16 hi + lo
-// of p * s_v have an absolute error of 2^-25 where the unit puts the tile's
-// largest scale into [2^14, 2^15).  While all scales are within 2^kSpan that is
-// 2^-27 of any weight's row at most, less than FP32 sums cost.  Past it (`wide`)
-// the unit has to be that of what a query row weighs: a large row that it does
-// not see, or next to nothing of, would take the others' bits.
-struct ScaleSpan {
-    static constexpr uint32_t kSpan = 12;
-    uint32_t top = 0u, low = 0x7f7fffffu;
-
-    // A lane's scale of the next tile, into `t` (largest) and `l` (smallest).
-    static __device__ __forceinline__ void look(float x, bool counts, uint32_t &t, uint32_t &l) {
-        const uint32_t b = __float_as_uint(x);
-        if (counts && b < 0x7f800000u) {
-            t = max(t, b);
-            l = min(l, b);
-        }
-    }
-    // The tile's largest, every lane's t and l taken in.
-    __device__ __forceinline__ float take(uint32_t t, uint32_t l) {
-        t = __reduce_max_sync(0xffffffffu, t);
-        top = max(top, t);
-        low = min(low, __reduce_min_sync(0xffffffffu, l));
-        return __uint_as_float(t);
-    }
-    // The same where each lane has one.
-    __device__ __forceinline__ float take(float x, bool counts) {
-        uint32_t t = 0u, l = 0x7f7fffffu;
-        look(x, counts, t, l);
-        return take(t, l);
-    }
-    __device__ __forceinline__ bool wide() const { return (top >> 23) > (low >> 23) + kSpan; }
-};
-
 // The maximum that a part of a split range leaves for the join, which leaves out
 // parts with -inf (nothing seen).  A running maximum passes NaN over, so a part that
 // saw nothing but NaN has -inf too: its sum says so, and the maximum becomes NaN.

@@ -14,9 +14,9 @@
 //  * Tensor-core sums are truncated, and a long run of them drifts towards
 //    zero; each tile is summed from zero and joins the FP32 output by an
 //    ordinary multiply-add.
-//  * p*s_v is scaled by a power of two for each tile so that FP16's range holds
-//    it whatever the scales are (for each query row and tile where they lie far
-//    apart: ScaleSpan); the same for each q row.
+//  * p*s_v is scaled by a power of two for each query row and tile, so that FP16
+//    holds the row's largest to 22 bits, whatever the scales are of what it does
+//    not see or hardly weighs; the same for each q row.
 #pragma once
 
 #include "q8.cuh"
@@ -107,10 +107,8 @@ struct TileMath {
     }
 
     // o, m, l of row g take the tile's rows; s is -inf where a row is not seen.
-    // top: the tile's largest scale; wide: ScaleSpan's.
-    static __device__ __forceinline__ void absorb(const unsigned char *sv, const float *svv, float top, bool wide,
-                                                  const float (&s)[NK / 8][2], float &m, float &l,
-                                                  float (&o)[NT][2]) {
+    static __device__ __forceinline__ void absorb(const unsigned char *sv, const float *svv, const float (&s)[NK / 8][2],
+                                                  float &m, float &l, float (&o)[NT][2]) {
         const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
         float mx = -INFINITY;
 #pragma unroll
@@ -121,42 +119,29 @@ struct TileMath {
         const float ref = mn == -INFINITY ? 0.f : mn;  // nothing seen so far
         const float alpha = fast_exp2(m - ref);
         m = mn;
-        // p * s_v in units of 2^(e-14), 2^e just above the tile's largest scale
-        const int e = max(int(__float_as_uint(top) >> 23), 15);
-        const float vup = __uint_as_float(uint32_t(268 - e) << 23);
-        float vdown = __uint_as_float(uint32_t(e - 14) << 23);
-        float w[NK / 8][2];
-        float sum = 0.f;
+        float w[NK / 8][2], sum = 0.f, most = 0.f;
 #pragma unroll
         for (int n = 0; n < NK / 8; ++n) {
             const float2 f = *reinterpret_cast<const float2 *>(svv + n * 8 + 2 * t);
             const float p0 = fast_exp2(s[n][0] - ref), p1 = fast_exp2(s[n][1] - ref);
             sum += p0 + p1;
             // a row that is not seen takes no part, whatever its scale
-            w[n][0] = s[n][0] == -INFINITY ? 0.f : p0 * (f.x * vup);
-            w[n][1] = s[n][1] == -INFINITY ? 0.f : p1 * (f.y * vup);
+            w[n][0] = s[n][0] == -INFINITY ? 0.f : p0 * f.x;
+            w[n][1] = s[n][1] == -INFINITY ? 0.f : p1 * f.y;
+            most = fmaxf(most, fmaxf(w[n][0], w[n][1]));
         }
-        if (__builtin_expect(wide, 0)) {  // the row's largest weight to [2^14, 2^15) (it is below that already)
-            float most = 0.f;
-#pragma unroll
-            for (int n = 0; n < NK / 8; ++n) most = fmaxf(most, fmaxf(w[n][0], w[n][1]));
-            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-            const int u = min(141 - int(__float_as_uint(most) >> 23), 120);
-            const float up = __uint_as_float(uint32_t(127 + u) << 23);
-            vdown *= __uint_as_float(uint32_t(127 - u) << 23);
-#pragma unroll
-            for (int n = 0; n < NK / 8; ++n) {
-                w[n][0] *= up;
-                w[n][1] *= up;
-            }
-        }
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        // the row's largest weight to [2^14, 2^15)
+        const int e = max(int(__float_as_uint(most) >> 23), 15);
+        const float vup = __uint_as_float(uint32_t(268 - e) << 23), vdown = __uint_as_float(uint32_t(e - 14) << 23);
         uint32_t hi[NK / 8], lo[NK / 8];
 #pragma unroll
         for (int n = 0; n < NK / 8; ++n) {
-            const __half2 h = __floats2half2_rn(w[n][0], w[n][1]);
+            const float w0 = w[n][0] * vup, w1 = w[n][1] * vup;
+            const __half2 h = __floats2half2_rn(w0, w1);
             const float2 b = __half22float2(h);
-            const __half2 r = __floats2half2_rn(w[n][0] - b.x, w[n][1] - b.y);
+            const __half2 r = __floats2half2_rn(w0 - b.x, w1 - b.y);
             hi[n] = *reinterpret_cast<const uint32_t *>(&h);
             lo[n] = *reinterpret_cast<const uint32_t *>(&r);
         }
