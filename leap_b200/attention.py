@@ -36,11 +36,15 @@ def rope_table(seq_len: int, head_dim: int, theta: float = 500000.0):
 _torch = None  # imported with the first device tensor
 
 
-def _dptr(t) -> int:
-    """Device pointer of a contiguous float32 CUDA tensor."""
+def _load_torch() -> None:
     global _torch
     if _torch is None:
         import torch as _torch
+
+
+def _dptr(t) -> int:
+    """Device pointer of a contiguous float32 CUDA tensor."""
+    _load_torch()
     torch = _torch
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise TypeError("expected a CUDA torch.Tensor")
@@ -61,8 +65,8 @@ def kv_kind(kv: str) -> int:
 def _ints(a, name: str, n: int | None = None) -> np.ndarray:
     """A 1-D host int32 array (kept as it is when it is one already) of whole
     numbers, none of which the conversion may change."""
-    a = np.asarray(a)
-    if a.dtype != np.int32:
+    if not isinstance(a, np.ndarray) or a.dtype != np.int32:
+        a = np.asarray(a)
         if a.size and (a.dtype.kind not in "iu" or a.min() < -2**31 or a.max() >= 2**31):
             raise ValueError(f"{name} must be whole numbers of 32 bits")
         a = a.astype(np.int32)
@@ -124,6 +128,7 @@ class AttentionContext:
         self.head_dim, self.max_seq, self.max_batch = head_dim, max_seq, max_batch
         self.device = device
         self.kv = kv
+        self._stream = self._raw = None  # the torch stream bound, if any, and its handle
         if bind_torch_stream:
             self.bind_torch_stream()
 
@@ -155,14 +160,30 @@ class AttentionContext:
     def bind_torch_stream(self, stream=None) -> None:
         """Order this context's work on a torch CUDA stream (default: the
         current stream of its device), so torch tensors can be passed
-        without extra synchronisation."""
+        without extra synchronisation.  Tensors that methods return belong to
+        that stream, whichever is current."""
         import torch
         if stream is None:
             stream = torch.cuda.current_stream(self.device)
         check(lib().leap_ctx_set_stream(self.handle, ctypes.c_void_p(stream.cuda_stream)))
+        self._stream, self._raw = stream, stream.cuda_stream
 
     def use_own_stream(self) -> None:
         check(lib().leap_ctx_use_own_stream(self.handle))
+        self._stream = self._raw = None
+
+    def _foreign(self) -> bool:
+        """Whether another stream than the bound one is current.  What methods
+        return is allocated on the stream that writes it: another stream's
+        allocator may hand out memory that work still queued there reads."""
+        return self._raw is not None and self._raw != _torch._C._cuda_getCurrentRawStream(self.device)
+
+    def _like(self, q):
+        _load_torch()
+        if self._foreign():
+            with _torch.cuda.stream(self._stream):
+                return _torch.empty_like(q)
+        return _torch.empty_like(q)
 
     def sync(self) -> None:
         check(lib().leap_sync(self.handle))
@@ -227,17 +248,22 @@ class AttentionContext:
                                  _iptr(n_keep), _iptr(nodes)))
 
     def _rows(self, n: int):
-        import torch
-        shape, dev = (max(n, 0), self.n_kv_heads, self.head_dim), torch.device("cuda", self.device)
-        return (torch.empty(shape, dtype=torch.float32, device=dev),
-                torch.empty(shape, dtype=torch.float32, device=dev))
+        _load_torch()
+        shape, dev = (max(n, 0), self.n_kv_heads, self.head_dim), _torch.device("cuda", self.device)
+        if self._raw is None:  # torch cannot order its memory on the context's own stream
+            _torch.cuda.current_stream(dev).synchronize()
+        elif self._foreign():
+            with _torch.cuda.stream(self._stream):
+                return (_torch.empty(shape, dtype=_torch.float32, device=dev),
+                        _torch.empty(shape, dtype=_torch.float32, device=dev))
+        return (_torch.empty(shape, dtype=_torch.float32, device=dev),
+                _torch.empty(shape, dtype=_torch.float32, device=dev))
 
     # -- attention ----------------------------------------------------------
     def decode(self, layer: int, pos: int, q, k_new, v_new, out=None):
         """Fused RoPE + append + attention for one token (device tensors)."""
-        import torch
         if out is None:
-            out = torch.empty_like(q)
+            out = self._like(q)
         check(lib().leap_attn_decode(self.handle, layer, pos, _dptr(q), _dptr(k_new),
                                      _dptr(v_new), _dptr(out)))
         return out
@@ -255,13 +281,12 @@ class AttentionContext:
 
     def decode_batched(self, layer: int, slots, positions, q, k_new, v_new, out=None):
         """Ragged batch: token i of slot slots[i] at positions[i]."""
-        import torch
         slots = np.ascontiguousarray(slots, np.int32)
         positions = np.ascontiguousarray(positions, np.int32)
         if slots.shape != positions.shape or slots.ndim != 1:
             raise ValueError("slots and positions must be equal-length 1-D")
         if out is None:
-            out = torch.empty_like(q)
+            out = self._like(q)
         check(lib().leap_attn_decode_batched(
             self.handle, layer, slots.shape[0], _iptr(slots), _iptr(positions), _dptr(q),
             _dptr(k_new), _dptr(v_new), _dptr(out)))
@@ -269,20 +294,18 @@ class AttentionContext:
 
     def prefill(self, slot: int, layer: int, pos0: int, q, k, v, out=None):
         """Causal prefill of q.shape[0] tokens starting at pos0."""
-        import torch
         if out is None:
-            out = torch.empty_like(q)
+            out = self._like(q)
         check(lib().leap_attn_prefill(self.handle, slot, layer, pos0, int(q.shape[0]),
                                       _dptr(q), _dptr(k), _dptr(v), _dptr(out)))
         return out
 
     def _packed(self, total: int, q, k, v, out):
         """Device pointers of a ragged call's tensors, their shapes checked."""
-        import torch
         qs, ks = (total, self.n_heads, self.head_dim), (total, self.n_kv_heads, self.head_dim)
         ptrs = [_dptr(q), _dptr(k), _dptr(v)]
         if out is None:
-            out = torch.empty_like(q)
+            out = self._like(q)
         ptrs.append(_dptr(out))
         for name, t, shape in (("q", q, qs), ("k", k, ks), ("v", v, ks), ("out", out, qs)):
             if t.shape != shape:
