@@ -981,6 +981,16 @@ void plan_tc(const leap_ctx *c, const Q8Seqs &tab, bool tree, Q8TcPlan &plan) {
 
 }  // namespace
 
+// Partials of 128 rows: four an SM, or every query tile of the longest runs in splits
+// of one key tile where that is less (plan_tc keeps to what there is).
+int q8_tc_parts_needed(const leap_ctx *c) {
+    const long splits = (long(c->max_seq) + kBN - 1) / kBN;
+    if (splits < 2) return 0;
+    const long tiles = (long(c->max_seq) * c->group + kBM - 1) / kBM;
+    const long all = std::min(c->max_batch, kMaxSeqPerLaunch) * c->n_kv * std::min(tiles, 1L << 20) * std::min(splits, 1L << 20);
+    return int(std::min(all, 4L * c->num_sms));
+}
+
 int q8_tc_attend(leap_ctx *c, int layer, const Q8Seqs &tab, const Q8Tree *tree, const float *q, const float *k,
                  const float *v, float *out) {
     Q8TcPlan plan;

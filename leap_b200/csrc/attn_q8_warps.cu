@@ -350,8 +350,11 @@ void plan_units(const leap_ctx *c, const Q8Seqs &tab, Q8Units &plan, int *longes
 
 }  // namespace
 
-// Two partials a warp.
-int q8_warps_parts(const leap_ctx *c) { return 2 * 2 * kWarps * c->num_sms; }
+// Two partials a warp, of those that a batch of the longest sequences has work for.
+int q8_warps_parts(const leap_ctx *c) {
+    const long units = long(std::min(c->max_batch, kMaxSeqPerLaunch)) * c->n_kv * ((c->max_seq + kTile - 1) / kTile + kPad);
+    return 2 * int(std::min((units + 1) / 2, long(2 * kWarps) * c->num_sms));  // plan_units: two units a warp at least
+}
 
 // What a batch costs here, in the unit of the rows kernel's plan (1/140 us with 128
 // dims): a warp's tiles, and one warp's join of the item in most parts, 8 of a row at a

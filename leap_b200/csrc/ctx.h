@@ -32,8 +32,10 @@ struct leap_ctx {
     uint8_t *k8 = nullptr, *v8 = nullptr;
     float *ks8 = nullptr, *vs8 = nullptr;
     size_t head_rows = 0, layer_rows = 0, slot_rows = 0;
-    float *d_rows = nullptr;  // FP32 rows on their way from or to host memory
-    // its split-KV scratch: partials of up to 8 rows, and tickets
+    float *d_rows = nullptr;  // FP32 rows on their way from or to host memory,
+    int stage_rows = 0;       // so many of k and of v
+    // its split-KV scratch, no more than the context can use: partials of up to 8
+    // rows, and tickets
     float *q8_part_o = nullptr, *q8_part_ml = nullptr;  // [q8_parts][8][hd], [q8_parts][8][2]
     unsigned *q8_counters = nullptr;                    // [kMaxSeqPerLaunch][n_kv]
     int q8_parts = 0;
@@ -152,7 +154,7 @@ int launch_prefill(leap_ctx *c, int slot, int layer, int pos0, int n_tok,
 // ---- 8-bit KV cache (kv_q8.cu, attn_q8*.cu) --------------------------------
 constexpr int kMaxTreeNodes = 128;     // nodes of one sequence's tree
 constexpr int kMaxNodesPerLaunch = 1024;  // (parameters of 2 KB)
-constexpr int kQ8StageRows = 1024;     // rows of k and v that d_rows holds
+constexpr int kQ8StageRows = 1024;     // rows of k and v that d_rows holds at most
 
 // A ragged batch of new tokens, by value in kernel parameters: sequence i has
 // packed tokens tok0[i] .. tok0[i+1]-1 behind pos[i] cached rows of its slot.
@@ -218,6 +220,7 @@ int kv_read_packed(leap_ctx *c, int layer, const Q8Seqs &tab, float *k, float *v
 // Move rows pos + at[j] to pos + j (j counted from each sequence's first).
 int kv_keep(leap_ctx *c, const Q8Seqs &tab, const Q8Nodes &nodes);
 int q8_warps_parts(const leap_ctx *c);
+int q8_tc_parts_needed(const leap_ctx *c);
 int q8_rows_attend(leap_ctx *c, int layer, const Q8Seqs &tab, const Q8Tree *tree, const float *q,
                    const float *k, const float *v, float *out);
 int q8_tc_attend(leap_ctx *c, int layer, const Q8Seqs &tab, const Q8Tree *tree, const float *q,

@@ -231,7 +231,8 @@ int q8_create(leap_ctx *c) {
     c->slot_rows = c->n_layers * c->layer_rows;
     const size_t rows = c->max_batch * c->slot_rows;
     c->q8_parts = q8_warps_parts(c);  // the rows kernel keeps to as many
-    c->q8_tc_parts = 4 * c->num_sms;
+    c->q8_tc_parts = q8_tc_parts_needed(c);
+    c->stage_rows = std::min(c->max_seq, kQ8StageRows);
     // two allocations (each costs a good part of a context's making): the cache, and
     // everything else; every piece a multiple of 256 bytes
     const size_t cache = 2 * rows * (c->hd + sizeof(float));
@@ -243,7 +244,7 @@ int q8_create(leap_ctx *c) {
     const size_t f = sizeof(float);
     const Piece pieces[] = {
         {reinterpret_cast<void **>(&c->q8_counters), size_t(kMaxSeqPerLaunch) * c->n_kv * sizeof(unsigned)},
-        {reinterpret_cast<void **>(&c->d_rows), 2 * f * kQ8StageRows * c->n_kv * c->hd},
+        {reinterpret_cast<void **>(&c->d_rows), 2 * f * c->stage_rows * c->n_kv * c->hd},
         {reinterpret_cast<void **>(&c->q8_part_o), f * c->q8_parts * kQ8Rows * c->hd},
         {reinterpret_cast<void **>(&c->q8_part_ml), f * c->q8_parts * kQ8Rows * 2},
         {reinterpret_cast<void **>(&c->q8_tc_part_o), f * c->q8_tc_parts * 128 * c->hd},
@@ -288,9 +289,9 @@ int q8_write(leap_ctx *c, int slot, int layer, int pos0, int n, const float *k, 
              bool from_host) {
     if (!from_host) return write_rows(c, layer, one_run(slot, pos0, n), k, v);
     const size_t row = size_t(c->n_kv) * c->hd;
-    float *dk = c->d_rows, *dv = dk + kQ8StageRows * row;
-    for (int r = 0; r < n; r += kQ8StageRows) {
-        const int m = n - r < kQ8StageRows ? n - r : kQ8StageRows;
+    float *dk = c->d_rows, *dv = dk + c->stage_rows * row;
+    for (int r = 0; r < n; r += c->stage_rows) {
+        const int m = std::min(n - r, c->stage_rows);
         const size_t bytes = m * row * sizeof(float);
         cudaError_t e = cudaMemcpyAsync(dk, k + r * row, bytes, cudaMemcpyHostToDevice, c->stream);
         if (e == cudaSuccess)
@@ -304,9 +305,9 @@ int q8_write(leap_ctx *c, int slot, int layer, int pos0, int n, const float *k, 
 int q8_read(leap_ctx *c, int slot, int layer, int pos0, int n, float *k, float *v, bool to_host) {
     if (!to_host) return launch_read(c, layer, one_run(slot, pos0, n), k, v);
     const size_t row = size_t(c->n_kv) * c->hd;
-    float *dk = c->d_rows, *dv = dk + kQ8StageRows * row;
-    for (int r = 0; r < n; r += kQ8StageRows) {
-        const int m = n - r < kQ8StageRows ? n - r : kQ8StageRows;
+    float *dk = c->d_rows, *dv = dk + c->stage_rows * row;
+    for (int r = 0; r < n; r += c->stage_rows) {
+        const int m = std::min(n - r, c->stage_rows);
         const size_t bytes = m * row * sizeof(float);
         if (int st = launch_read(c, layer, one_run(slot, pos0 + r, m), dk, dv)) return st;
         cudaError_t e = cudaMemcpyAsync(k + r * row, dk, bytes, cudaMemcpyDeviceToHost, c->stream);
