@@ -65,11 +65,15 @@ def kv_kind(kv: str) -> int:
 def _ints(a, name: str, n: int | None = None) -> np.ndarray:
     """A 1-D host int32 array (kept as it is when it is one already) of whole
     numbers, none of which the conversion may change."""
-    if not isinstance(a, np.ndarray) or a.dtype != np.int32:
-        a = np.asarray(a)
-        if a.size and (a.dtype.kind not in "iu" or a.min() < -2**31 or a.max() >= 2**31):
+    if isinstance(a, list) and all(type(x) is int and -2**31 <= x < 2**31 for x in a):
+        a = np.array(a, np.int32)
+    elif not isinstance(a, np.ndarray) or a.dtype != np.int32:
+        wide = np.asarray(a)
+        if wide.size and wide.dtype.kind not in "iu":
             raise ValueError(f"{name} must be whole numbers of 32 bits")
-        a = a.astype(np.int32)
+        a = wide.astype(np.int32)
+        if (a != wide).any():
+            raise ValueError(f"{name} must be whole numbers of 32 bits")
     a = np.ascontiguousarray(a)
     if a.ndim != 1 or (n is not None and a.shape[0] != n):
         raise ValueError(f"{name} must be 1-D" + ("" if n is None else f" of length {n}"))
