@@ -9,8 +9,8 @@
 // an item ends it stages the next item's queries and leaves its part of the sums,
 // or the output, alone: no block ever waits for its warps, so the other 15 of an
 // SM keep the copies going.  64 sequences of 512 to 8192 rows, 8 kv heads of 128:
-// 105 us, 5.45 TB/s; blocks that walked such a list together lost about 9 us an item
-// to their joins (141 us).  The parts of an item are joined by the warp that is last (atomic
+// 106 us one launch after another, 112 us where nothing is in the L2 (5.1 TB/s); blocks
+// that walked such a list together lost about 9 us an item to their joins (141 us).  The parts of an item are joined by the warp that is last (atomic
 // ticket).  The products are those of q8_tile.cuh.
 //
 // New rows are appended by the warp that reads the tile they fall in, before it
