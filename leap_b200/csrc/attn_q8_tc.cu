@@ -73,7 +73,7 @@ struct TcArgs {
     const float *rope_cos, *rope_sin;
     float *part_o, *part_ml;  // [parts][128][HD], [parts][128][2]
     int *err;
-    float scale_log2;
+    float scale;  // 2^-14 log2(e) / sqrt(HD), taken into the scales of K
 };
 
 struct TcBars {
@@ -328,7 +328,9 @@ q8_tc_kernel(const __grid_constant__ TcArgs a, const __grid_constant__ Q8Seqs ta
                     *reinterpret_cast<uint32_t *>(qs) = hi[0];
                     *reinterpret_cast<uint32_t *>(qs + kBM * C::kQRow) = lo[0];
                 }
-                fac_of_lane = lane == u ? __uint_as_float(uint32_t(ex - 14) << 23) * a.scale_log2 : fac_of_lane;
+                // A power of two, so that score * fac is exact and the largest key's
+                // exponent is 0, however large the scores are.
+                fac_of_lane = lane == u ? __uint_as_float(uint32_t(ex) << 23) : fac_of_lane;
             }
             if (lane < U) s_fac[warp + 8 * lane] = fac_of_lane;
         }
@@ -654,7 +656,7 @@ q8_tc_kernel(const __grid_constant__ TcArgs a, const __grid_constant__ Q8Seqs ta
                 }
                 const int e = max(int(__float_as_uint(span.take(t, l)) >> 23), 15);
                 const float vup = __uint_as_float(uint32_t(268 - e) << 23);
-                s_ks[slot][ct] = ct < n ? gks[first + ct] : 0.f;
+                s_ks[slot][ct] = ct < n ? gks[first + ct] * a.scale : 0.f;
                 s_vs[slot][ct] = ct < n ? gvs[first + ct] * vup : 0.f;
                 if (ct == 0) s_vdown[slot] = __uint_as_float(uint32_t(e - 14) << 23 | (span.wide() ? 0x80000000u : 0u));
                 __syncwarp();
@@ -1020,7 +1022,7 @@ int q8_tc_attend(leap_ctx *c, int layer, const Q8Seqs &tab, const Q8Tree *tree, 
     a.part_o = c->q8_tc_part_o;
     a.part_ml = c->q8_tc_part_ml;
     a.err = c->d_err;
-    a.scale_log2 = kLog2e / sqrtf(float(c->hd));
+    a.scale = kLog2e / (16384.f * sqrtf(float(c->hd)));
     switch (c->hd * 100 + c->group) {
         case 12801: return launch_tc_g<128, 1>(c, a, tab, plan, tree);
         case 12802: return launch_tc_g<128, 2>(c, a, tab, plan, tree);

@@ -112,3 +112,37 @@ def test_bad_value_whose_weight_vanishes(cuda, shape, n):
         out = ctx.decode_tree(0, [0], [rows], [n], par, *gpu(q, k, v)).cpu().numpy()
         check_rows(ctx, out, stored(k0), stored(v0), q, k, v, par, terms=50)
         assert np.isnan(out[:, h // kv:2 * (h // kv)]).all()
+
+
+@pytest.mark.parametrize("size", [1e30, 1e33, 1e36])
+@pytest.mark.parametrize("shape,n", [("l8b", 1), ("l8b", 2), ("l8b", 40), ("mha64", 120), ("tl", 3)])
+def test_keys_far_beyond_the_others(cuda, shape, n, size):
+    """Scores that FP32 holds (up to 1e38 here) take all the weight, or none."""
+    rng = np.random.default_rng(54)
+    h, kv, hd = ALL[shape]
+    rows = 300
+    with make(shape, rows + n) as ctx:
+        k0, v0 = rnd(rng, rows, kv, hd), rnd(rng, rows, kv, hd)
+        k0[77] *= np.float32(size)
+        ctx.kv_write(0, 0, 0, k0, v0)
+        q, k, v = rnd(rng, n, h, hd), rnd(rng, n, kv, hd), rnd(rng, n, kv, hd)
+        par = tree(rng, n)
+        out = ctx.decode_tree(0, [0], [rows], [n], par, *gpu(q, k, v)).cpu().numpy()
+        check_rows(ctx, out, stored(k0), stored(v0), q, k, v, par)
+
+
+@pytest.mark.parametrize("shape,n", [("l8b", 2), ("l8b", 40), ("mha64", 120)])
+def test_small_keys_under_large_queries(cuda, shape, n):
+    """Scores of ordinary size from factors that are not."""
+    rng = np.random.default_rng(55)
+    h, kv, hd = ALL[shape]
+    rows = 300
+    for up in (1e25, 1e-25):
+        with make(shape, rows + n) as ctx:
+            down = np.float32(1 / up)
+            k0, v0 = rnd(rng, rows, kv, hd) * down, rnd(rng, rows, kv, hd)
+            ctx.kv_write(0, 0, 0, k0, v0)
+            q, k, v = rnd(rng, n, h, hd) * np.float32(up), rnd(rng, n, kv, hd) * down, rnd(rng, n, kv, hd)
+            par = tree(rng, n)
+            out = ctx.decode_tree(0, [0], [rows], [n], par, *gpu(q, k, v)).cpu().numpy()
+            check_rows(ctx, out, stored(k0), stored(v0), q, k, v, par)
