@@ -125,3 +125,18 @@ def test_decode_of_many_with_large_values_of_little_weight(cuda):
             out = out.cpu().numpy()
             for s in range(0, n, 9):
                 check_rows(ctx, out[s:s + 1], stored(k0), stored(v0), q, k, v, terms=45)
+
+
+@pytest.mark.parametrize("size", [1e-35, 1e-20, 1e20, 1e36])
+@pytest.mark.parametrize("shape,n", [("l8b", 1), ("mha128", 8), ("l8b", 40), ("tl", 128)])
+def test_values_all_tiny_or_all_large(cuda, shape, n, size):
+    rng = np.random.default_rng(66)
+    h, kv, hd = ALL[shape]
+    rows = 400
+    with make(shape, rows + n) as ctx:
+        k0, v0 = rnd(rng, rows, kv, hd), rnd(rng, rows, kv, hd) * np.float32(size)
+        ctx.kv_write(0, 0, 0, k0, v0)
+        q, k, v = rnd(rng, n, h, hd), rnd(rng, n, kv, hd), rnd(rng, n, kv, hd) * np.float32(size)
+        par = tree(rng, n)
+        out = ctx.decode_tree(0, [0], [rows], [n], par, *gpu(q, k, v)).cpu().numpy()
+        check_rows(ctx, out, stored(k0), stored(v0), q, k, v, par)
