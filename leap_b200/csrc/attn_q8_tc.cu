@@ -643,6 +643,13 @@ q8_tc_kernel(const __grid_constant__ TcArgs a, const __grid_constant__ Q8Seqs ta
             const int b = j & 1, slot = j & (kSlots - 1);
             if (j >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&bars.s_full[b], par(j - 2)));
             if (!ok) break;
+            store(C::kK + b * C::kOp, 0);
+            load(gv, j, 0);
+            store(C::kK + b * C::kOp, 1);
+            load(gv, j, 1);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars.k_full[b]);
             // Scales (of rows the block may see; the others count as 0).  Slot
             // j % 4 was last read for tile j - 4: S(j-2) was issued after
             // PV(j-4), that after the softmax of tile j-4.
@@ -662,13 +669,6 @@ q8_tc_kernel(const __grid_constant__ TcArgs a, const __grid_constant__ Q8Seqs ta
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bars.sc_full[slot]);
             }
-            store(C::kK + b * C::kOp, 0);
-            load(gv, j, 0);
-            store(C::kK + b * C::kOp, 1);
-            load(gv, j, 1);
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bars.k_full[b]);
             if (j >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&bars.o_full[b], par(j - 2)));
             if (!ok) break;
             if (j + 1 < n_kt) settle(j + 1);
