@@ -117,8 +117,8 @@ __device__ __forceinline__ Item item_of(const Q8TcPlan &plan, int n_kv, int bloc
 // the unit has to be that of what a query row weighs: a large row that it does
 // not see, or next to nothing of, would take the others' bits.  Rows of zeros count
 // as far apart, since one can hold nearly all of a query's weight.  That costs an
-// exchange between the two threads of a row (prompt of 8192: 1132 us a call narrow,
-// 1599 wide; 8 ragged trees 93, 142), the record itself 1% (1014 -> 1025 us).
+// exchange between the two threads of a row (prompt of 8192: 1116 us a call narrow,
+// 1617 wide; 8 ragged trees 93, 142).
 struct ScaleSpan {
     static constexpr uint32_t kSpan = 12;
     uint32_t top = 0u, low = 0x7f7fffffu;

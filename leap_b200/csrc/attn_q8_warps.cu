@@ -9,7 +9,7 @@
 // an item ends it stages the next item's queries and leaves its part of the sums,
 // or the output, alone: no block ever waits for its warps, so the other 15 of an
 // SM keep the copies going.  64 sequences of 512 to 8192 rows, 8 kv heads of 128:
-// 106 us one launch after another, 112 us where nothing is in the L2 (5.1 TB/s); blocks
+// 106 us one launch after another, 112 to 114 us where nothing is in the L2 (5.1 TB/s); blocks
 // that walked such a list together lost about 9 us an item to their joins (141 us).  The parts of an item are joined by the warp that is last (atomic
 // ticket).  The products are those of q8_tile.cuh.
 //
